@@ -98,6 +98,13 @@ SIGNATURES: dict[str, tuple] = {
     "ferrite_adamw_step": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _f32, _f32, _f32, _f32, _i64, _f32, _f32, _vp, _vp, _sz]),
     "ferrite_xent_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32]),
     "ferrite_xent_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _f32, _vp, _i64, _i64, _i64, _i64, _i32, _i32]),
+    "ferrite_logprobs_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _i32, _i32]),
+    "ferrite_logprobs_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _i32]),
+    "ferrite_policy_loss": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _f32, _f32, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                   _sz, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32]),
+    "ferrite_preference_pairs": (_i32, [_vp, _vp, _vp, _vp, _vp, _f32, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i32]),
+    "ferrite_distill_loss": (_i32, [_vp, _vp, _vp, _vp, _vp, _f32, _vp, _f32, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
+                                    _i32, _i32, _i32]),
     "ferrite_attn_bwd_ds_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32]),
     "ferrite_attn_bwd_ds": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sp, _vp, _sz, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _i32, _i32]),
     "ferrite_attn_bwd_dkv_ds": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _i32, _i32]),

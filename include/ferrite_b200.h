@@ -254,6 +254,84 @@ FERRITE_API int ferrite_xent_bwd(void* stream, const float* logits, const void* 
                      int64_t rows, int64_t vocab, int64_t ld, int64_t ld_out,
                      int target_dtype, int out_dtype);
 
+/* ---- losses over given tokens: policy, preference, distillation ------------------ */
+
+/* The losses that follow pre-training, over the same logits as ferrite_xent_*.  No
+ * counterpart in the reference, whose only loss is the mean cross-entropy of
+ * loss_fn (model/gpt.py:147-152).  Shared by the entry points below:
+ *   - logits [rows, vocab] of `dtype` (f32, bf16 or f16) with row stride ld; z = logits /
+ *     temperature, p = softmax(z), logp_r = log p[target_r], H_r = -sum p log p.
+ *   - targets int32 (target_dtype 0) or int64 (1).  A row whose target is ignore_index
+ *     is masked: its logits are not read, its results and its gradient are zeros.  Any
+ *     other target outside [0, vocab) gives NaN for the row; nothing is read or written
+ *     out of range.
+ *   - dlogits [rows, vocab] of `out_dtype` (dtype itself, or bf16 / f16 for f32 logits)
+ *     with row stride ld_out; it must not overlap logits.  The gradient is that of the loss
+ *     times (*dloss) * scale (dloss a device scalar, NULL meaning 1).
+ *   - statistics, sums and losses are f32 (sums over rows are accumulated in f64, in a
+ *     fixed order: results do not change from run to run).
+ *   - a logit of -inf has p = 0 exactly; NaN or +inf makes the row's results NaN. */
+
+/* logp [rows] and, when entropy is given, H [rows].  stats (may be NULL) takes 2 floats
+ * a row for the backward. */
+FERRITE_API int ferrite_logprobs_fwd(void* stream, const void* logits, const void* targets, float* logp,
+                        float* entropy, float* stats, int64_t rows, int64_t vocab, int64_t ld,
+                        int64_t ignore_index, float temperature, int dtype, int target_dtype);
+
+/* dlogits of sum_r dlogp_r logp_r + dentropy_r H_r (either may be NULL: zero), from the
+ * forward's stats and, with dentropy, its entropy. */
+FERRITE_API int ferrite_logprobs_bwd(void* stream, const void* logits, const void* targets, const float* stats,
+                        const float* entropy, const float* dlogp, const float* dentropy,
+                        const float* dloss, float scale, void* dlogits, int64_t rows, int64_t vocab,
+                        int64_t ld, int64_t ld_out, int64_t ignore_index, float temperature,
+                        int dtype, int target_dtype, int out_dtype);
+
+/* The clipped policy loss, and in the same pass its gradient when dlogits is given:
+ *   ratio = exp(logp - old_logp), pg = -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A),
+ *   kl = exp(ref_logp - logp) - (ref_logp - logp) - 1   (0 when ref_logp is NULL),
+ *   *loss = sum_r w_r (pg_r + kl_coef kl_r - entropy_coef H_r).
+ * weights [rows] (NULL: 1 / rows); a row of weight 0 is masked like one of ignore_index.
+ * logp, entropy, kl, clipped (1 where the clipped branch is the smaller) are written per
+ * row.  workspace: rows floats. */
+FERRITE_API int ferrite_policy_loss(void* stream, const void* logits, const void* targets, const float* old_logp,
+                        const float* advantages, const float* weights, const float* ref_logp,
+                        float clip_low, float clip_high, float kl_coef, float entropy_coef,
+                        float temperature, const float* dloss, float scale, float* loss, float* logp,
+                        float* entropy, float* kl, uint8_t* clipped, void* dlogits, float* workspace,
+                        size_t workspace_bytes, int64_t rows, int64_t vocab, int64_t ld, int64_t ld_out,
+                        int64_t ignore_index, int dtype, int target_dtype, int out_dtype);
+
+/* The preference loss of `pairs` pairs of sequences, from the rows' logp.  Sequence j owns
+ * rows [offsets[j], offsets[j + 1]) (int64 [2 pairs + 1] on the device, non-decreasing;
+ * values outside [0, rows] are clamped); 2p is pair p's chosen sequence, 2p + 1 its
+ * rejected one.  Masked rows (ignore_index) count in no sequence.
+ *   d_j = sum of (logp - ref_logp) over the sequence (average != 0: divided by its rows),
+ *   h = d_2p - d_2p+1, s = sigmoid, e = label_smoothing,
+ *   kind 0: -(1 - e) log s(beta h) - e log s(-beta h);  1: (h - 1 / (2 beta))^2;
+ *   kind 2: max(0, 1 - beta h);  *loss = the mean over pairs, margins[p] = beta h.
+ * coef [rows] (may be NULL) is dloss/dlogp, ferrite_logprobs_bwd's dlogp.  workspace: pairs
+ * floats. */
+FERRITE_API int ferrite_preference_pairs(void* stream, const float* logp, const float* ref_logp,
+                        const void* targets, const int64_t* offsets, float beta,
+                        float label_smoothing, int kind, int average, float* loss, float* margins,
+                        float* coef, float* workspace, size_t workspace_bytes, int64_t rows,
+                        int64_t pairs, int64_t ignore_index, int target_dtype);
+
+/* Distillation from a teacher's top logits, and in the same pass its gradient when
+ * dlogits is given: values (value_dtype) and indices (index_dtype 0 int32, 1 int64) are
+ * [rows, top] lists with row stride ld_list, 1 <= top <= 1024.
+ *   q = softmax(values / temperature) over the row's entries, per_token = temperature^2
+ *   sum_j q_j (log q_j - log p[indices_j]), *loss = sum_r w_r per_token_r.
+ * An entry with a negative index or the value -inf is absent; a row without entries, or of
+ * weight 0, is masked.  An index >= vocab gives NaN for the row.  A token listed twice
+ * counts with both weights.  weights [rows] (NULL: 1 / rows).  workspace: rows floats. */
+FERRITE_API int ferrite_distill_loss(void* stream, const void* logits, const void* values, const void* indices,
+                        const float* weights, float temperature, const float* dloss, float scale,
+                        float* loss, float* per_token, void* dlogits, float* workspace,
+                        size_t workspace_bytes, int64_t rows, int64_t vocab, int64_t top, int64_t ld,
+                        int64_t ld_out, int64_t ld_list, int dtype, int value_dtype, int index_dtype,
+                        int out_dtype);
+
 /* ---- AdamW over flat parameters --------------------------------------------- */
 
 /* Bytes of scratch ferrite_adamw_step needs for n elements (the grad-norm
