@@ -114,6 +114,8 @@ static __device__ int g_device_status = 0;
 int status_gemm(int clear);
 int status_attention(int clear);
 int status_rmsnorm(int clear);
+int status_logprobs(int clear);
+int status_distill(int clear);
 
 // --------------------------------------------------------------------------
 // device: dtype helpers

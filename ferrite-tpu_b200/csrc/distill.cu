@@ -13,7 +13,7 @@ namespace rowloss {
 constexpr int kMaxTop = 1024;
 
 struct Distill {
-  static constexpr bool kEnt = false, kGradEnt = false, kHasStats = false;
+  static constexpr bool kEnt = false, kGradEnt = false, kHasStats = false, kList = true, kForwardOnly = false;
   const void* values;   // [rows, top] teacher logits
   const void* indices;  // [rows, top]
   int64_t ld_list;
@@ -23,22 +23,29 @@ struct Distill {
   float* terms;      // [rows] w * tau^2 * KL
   float* per_token;  // [rows] tau^2 * KL
 
-  // Shared memory: q, the student's logits at the listed tokens, the tokens, and the row's summary.
-  struct Shared {
+  struct Pre {
+    float w;
+  };
+  // A row in shared memory: this, then q, the student's logits at the listed tokens, the tokens.
+  struct Row {
+    float w;
+    float qlogq;  // sum_j q_j log2 q_j
+    float bad;    // NaN if an index is out of range
+    int entries;  // 0: a masked row
+  };
+  struct List {
     float* q;
     float* x;
     int* idx;
-    float* info;  // [0] sum_j q_j log2 q_j, [1] entries (0: masked row), [2] NaN if an index is out of range
   };
-  __device__ Shared shared(char* sh) const {
-    Shared s;
-    s.q = reinterpret_cast<float*>(sh);
-    s.x = s.q + top;
-    s.idx = reinterpret_cast<int*>(s.x + top);
-    s.info = reinterpret_cast<float*>(s.idx + top);
-    return s;
+  __host__ __device__ int slot_bytes() const { return (int)sizeof(Row) + top * 12; }
+  __device__ List list(char* slot) const {
+    List l;
+    l.q = reinterpret_cast<float*>(slot + sizeof(Row));
+    l.x = l.q + top;
+    l.idx = reinterpret_cast<int*>(l.x + top);
+    return l;
   }
-  static size_t shared_bytes(int top) { return (size_t)top * 12 + 16; }
 
   __device__ float value(int64_t i) const {
     if (value_dtype == FERRITE_F32) return static_cast<const float*>(values)[i];
@@ -48,30 +55,28 @@ struct Distill {
   __device__ int64_t index(int64_t i) const {
     return index64 ? static_cast<const int64_t*>(indices)[i] : (int64_t) static_cast<const int32_t*>(indices)[i];
   }
-  __device__ float weight(int64_t r) const { return weights ? weights[r] : uniform; }
-  __device__ bool live(int64_t r) const { return weight(r) != 0.f; }
+  __device__ Pre pre(int64_t r) const { return Pre{weights ? weights[r] : uniform}; }
+  __device__ bool live(const Pre& p) const { return p.w != 0.f; }
   __device__ void dead(int64_t r) const { terms[r] = per_token[r] = 0.f; }
 
-  // Warp 0: the teacher's softmax over the list and the student's logits there.
+  // The teacher's softmax over the list, and the student's logits there.
   template <typename TI>
-  __device__ void begin(int64_t r, const TI* x, int n, char* sh) const {
-    if (threadIdx.x >= 32) return;
-    const Shared s = shared(sh);
-    const int lane = threadIdx.x;
-    const float k = kLog2e / tau;
+  __device__ void prep(int64_t r, const Pre& p, const TI* x, const RowIn& in, char* slot) const {
+    const List l = list(slot);
+    const int lane = threadIdx.x & 31;
     float m = -INFINITY, bad = 0.f;
     int count = 0;
     for (int j = lane; j < top; j += 32) {
       int64_t i = index(r * ld_list + j);
-      float v = value(r * ld_list + j);
+      const float v = value(r * ld_list + j);
       if (v == -INFINITY) i = -1;
-      if (i >= n) bad = __int_as_float(0x7fc00000), i = -1;
-      s.idx[j] = i < 0 ? -1 : (int)i;
-      s.x[j] = i < 0 ? 0.f : DT<TI>::to_f(x[i]);
-      s.q[j] = v;
+      if (i >= in.vocab) bad = __int_as_float(0x7fc00000), i = -1;
+      l.idx[j] = i < 0 ? -1 : (int)i;
+      l.x[j] = i < 0 ? 0.f : DT<TI>::to_f(x[i]);
+      l.q[j] = v;
       if (i >= 0) {
         ++count;
-        m = v != v ? v : fmaxf(m, v);  // a NaN value shows through the sums
+        m = fmaxf(m, v);  // a NaN value shows through the sums
       }
     }
 #pragma unroll
@@ -82,9 +87,9 @@ struct Distill {
     }
     float sum = 0.f, dot = 0.f;
     for (int j = lane; j < top; j += 32) {
-      const float y = (s.q[j] - m) * k;
-      const float e = s.idx[j] >= 0 ? ex2_approx(y) : 0.f;
-      s.q[j] = e;
+      const float y = (l.q[j] - m) * in.k;
+      const float e = l.idx[j] >= 0 ? ex2_approx(y) : 0.f;
+      l.q[j] = e;
       sum += e;
       dot += e > 0.f ? e * y : (e != e ? e : 0.f);
     }
@@ -93,58 +98,56 @@ struct Distill {
       sum += __shfl_xor_sync(0xffffffffu, sum, off);
       dot += __shfl_xor_sync(0xffffffffu, dot, off);
     }
-    for (int j = lane; j < top; j += 32) s.q[j] /= sum;
-    if (lane == 0) {
-      s.info[0] = dot / sum - log2f(sum);  // sum_j q_j log2 q_j
-      s.info[1] = (float)count;
-      s.info[2] = bad;
-    }
+    for (int j = lane; j < top; j += 32) l.q[j] /= sum;
+    if (lane == 0) *reinterpret_cast<Row*>(slot) = Row{p.w, dot / sum - log2f(sum), bad, bad != bad ? max(count, 1) : count};
   }
-  template <typename TI>
-  __device__ Coef finish(int64_t r, const State& st, const TI*, const RowIn& in, float g, bool writer, char* sh) const {
-    const Shared s = shared(sh);
-    const float w = weight(r);
-    const bool any = s.info[1] > 0.f || s.info[2] != s.info[2];
-    const float bad = s.info[2];
-    if (writer && threadIdx.x < 32) {
-      const float c = st.m * in.k, ls = log2f(st.s);
+  __device__ Coef finish(int64_t r, const Norm& w, const RowIn& in, float g, bool writer, char* slot) const {
+    const List l = list(slot);
+    const Row row = *reinterpret_cast<const Row*>(slot);
+    Coef cf;
+    const float scale = grad_base(w, in, cf) / w.s;
+    if (writer) {
+      const int lane = threadIdx.x & 31;
+      const float ls = log2f(w.s);
       float part = 0.f;
-      for (int j = threadIdx.x; j < top; j += 32)
-        if (s.idx[j] >= 0 && s.q[j] != 0.f) part += s.q[j] * (y_of(s.x[j], in.k, st.m, c) - ls);
+      for (int j = lane; j < top; j += 32)
+        if (l.idx[j] >= 0 && l.q[j] != 0.f) part += l.q[j] * (y_of(l.x[j], w, in) - ls);
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) part += __shfl_xor_sync(0xffffffffu, part, off);
-      if (threadIdx.x == 0) {
-        const float per = any ? tau * tau * kLn2 * (s.info[0] - part) + bad : 0.f;
+      if (lane == 0) {
+        const float per = row.entries ? tau * tau * kLn2 * (row.qlogq - part) + row.bad : 0.f;
         per_token[r] = per;
-        terms[r] = any ? w * per : 0.f;
+        terms[r] = row.entries ? row.w * per : 0.f;
       }
     }
-    const float f = w * tau * g + bad;
-    Coef cf;
-    cf.A = f / st.s;
+    const float f = row.w * tau * g + row.bad;
+    cf.A = f * scale;
     cf.B = 0.f;
     cf.at_t = -f;
-    cf.masked = !any;
+    cf.t = -1;
+    cf.masked = row.entries == 0;
     return cf;
   }
-  // The listed tokens' entries in [lo, hi): the thread of entry j sums the weights of every entry
-  // with the same token, so that a token listed twice is written the same value twice.
-  template <typename TO, typename TI>
-  __device__ void fix(int64_t, const State& st, const Coef& cf, TO* dx, int lo, int hi, const TI*, const RowIn& in, float, char* sh) const {
-    const Shared s = shared(sh);
-    if (!(s.info[1] > 0.f)) return;
-    const float c = st.m * in.k;
-    for (int j = threadIdx.x; j < top; j += blockDim.x) {
-      const int i = s.idx[j];
-      if (i < lo || i >= hi) continue;
+  // The listed tokens' entries in [lo, hi), by threads tid < threads: the thread of entry j sums the
+  // weights of every entry with the same token, so that a token listed twice is written the same
+  // value twice.
+  template <typename TO>
+  __device__ void fix(const Coef& cf, TO* dx, int lo, int hi, const RowIn& in, char* slot, int tid, int threads) const {
+    const List l = list(slot);
+    for (int j = tid; j < top; j += threads) {
+      const int i = l.idx[j];
+      if (i < lo || i >= hi) continue;  // absent entries too: lo is not negative
       float q = 0.f;
-      for (int l = 0; l < top; ++l) q += s.idx[l] == i ? s.q[l] : 0.f;
-      dx[i] = DT<TO>::from_f(fmaf(cf.at_t, q, grad_of<false>(s.x[j], in.k, st.m, c, is_big(c), cf.A, 0.f)));
+      for (int o = 0; o < top; ++o) q += l.idx[o] == i ? l.q[o] : 0.f;
+      dx[i] = DT<TO>::from_f(fmaf(cf.at_t, q, grad_of<false>(l.x[j], in.k, cf)));
     }
   }
 };
 
 }  // namespace rowloss
+
+FERRITE_DEFINE_STATUS_READER(status_distill)
+
 }  // namespace ferrite
 
 using namespace ferrite;
@@ -171,10 +174,10 @@ int ferrite_distill_loss(void* stream, const void* logits, const void* values, c
     if (!logits || !values || !indices || !per_token || !workspace) return fail(FERRITE_BAD_SHAPE, "%s: null pointer", op);
     if (misaligned(logits, elem_bytes(dtype)) || (dlogits && misaligned(dlogits, elem_bytes(out_dtype))))
       return fail(FERRITE_BAD_ALIGNMENT, "%s: misaligned pointer", op);
-    const RowIn in{logits, rows, vocab, ld, kLog2e / temperature, 1.f / temperature};
+    const RowIn in = row_in(logits, rows, vocab, ld, temperature);
     const RowOut out{dlogits, ld_out, dloss, scale};
     const Distill d{values, indices, ld_list, (int)top, value_dtype, index_dtype, weights, 1.f / (float)rows, temperature, workspace, per_token};
-    if (int rc = dispatch_row(s, in, out, d, dtype, dlogits ? out_dtype : -1, Distill::shared_bytes((int)top), op)) return rc;
+    if (int rc = dispatch_row(s, in, out, d, dtype, dlogits ? out_dtype : -1, op)) return rc;
   }
   return sum_terms(s, workspace, loss, rows, 1.f, op);
 }

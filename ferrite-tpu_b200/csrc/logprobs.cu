@@ -12,87 +12,92 @@
 namespace ferrite {
 namespace rowloss {
 
-// Target handling shared by the ops below: the logit there, and what a row whose
-// target lies outside [0, vocab) gives (NaN; nothing is read or written out of range).
+// The logit at the target; a target outside [0, vocab) gives NaN (nothing is read out of range).
 template <typename TI>
 __device__ __forceinline__ float logit_at(const TI* x, int64_t t, int64_t n) {
   return t >= 0 && t < n ? DT<TI>::to_f(x[t]) : __int_as_float(0x7fc00000);
 }
-__device__ __forceinline__ float logp_of(float xt, const State& st, float k) {
-  return (y_of(xt, k, st.m, st.m * k) - log2f(st.s)) * kLn2;
-}
-__device__ __forceinline__ float entropy_of(const State& st) { return (log2f(st.s) - st.u / st.s) * kLn2; }
-
-template <bool ENT, typename TO, typename TI>
-__device__ __forceinline__ void fix_target(int64_t t, const State& st, const Coef& cf, TO* dx, int lo, int hi, const TI* x, const RowIn& in) {
-  if (threadIdx.x == 0 && t >= lo && t < hi) {
-    const float c = st.m * in.k;
-    dx[t] = DT<TO>::from_f(grad_of<ENT>(DT<TI>::to_f(x[t]), in.k, st.m, c, is_big(c), cf.A, cf.B) + cf.at_t);
-  }
-}
 
 template <bool ENT>
 struct LogprobsFwd {
-  static constexpr bool kEnt = ENT, kGradEnt = false, kHasStats = false;
+  static constexpr bool kEnt = ENT, kGradEnt = false, kHasStats = false, kList = false, kForwardOnly = true;
   Targets t;
   float* logp;
   float* entropy;
   float2* stats;
-  __device__ bool live(int64_t r) const { return t.at(r) != t.ignore; }
+  struct Pre {
+    int64_t t;
+  };
+  struct Row {
+    float xt;
+  };
+  __host__ __device__ int slot_bytes() const { return sizeof(Row); }
+  __device__ Pre pre(int64_t r) const { return Pre{t.at(r)}; }
+  __device__ bool live(const Pre& p) const { return p.t != t.ignore; }
   __device__ void dead(int64_t r) const {
     logp[r] = 0.f;
     if constexpr (ENT) entropy[r] = 0.f;
     if (stats) stats[r] = make_float2(0.f, 1.f);
   }
   template <typename TI>
-  __device__ void begin(int64_t, const TI*, int, char*) const {}
-  template <typename TI>
-  __device__ Coef finish(int64_t r, const State& st, const TI* x, const RowIn& in, float, bool writer, char*) const {
-    if (writer && threadIdx.x == 0) {
-      logp[r] = logp_of(logit_at(x, t.at(r), in.vocab), st, in.k);
-      if constexpr (ENT) entropy[r] = entropy_of(st);
-      if (stats) stats[r] = make_float2(st.m, st.s);
+  __device__ void prep(int64_t, const Pre& p, const TI* x, const RowIn& in, char* slot) const {
+    if ((threadIdx.x & 31) == 0) reinterpret_cast<Row*>(slot)->xt = logit_at(x, p.t, in.vocab);
+  }
+  __device__ Coef finish(int64_t r, const Norm& w, const RowIn& in, float, bool writer, char* slot) const {
+    if (writer && (threadIdx.x & 31) == 0) {
+      logp[r] = logp_of(reinterpret_cast<Row*>(slot)->xt, w, in);
+      if constexpr (ENT) entropy[r] = entropy_of(w);
+      if (stats) stats[r] = make_float2(w.base, w.big ? -w.s : w.s);
     }
     return Coef{};
   }
-  template <typename TO, typename TI>
-  __device__ void fix(int64_t, const State&, const Coef&, TO*, int, int, const TI*, const RowIn&, float, char*) const {}
 };
 
 template <bool ENT>
 struct LogprobsBwd {
-  static constexpr bool kEnt = false, kGradEnt = ENT, kHasStats = true;
+  static constexpr bool kEnt = false, kGradEnt = ENT, kHasStats = true, kList = false, kForwardOnly = false;
   Targets t;
   const float2* stats;
   const float* entropy;   // ENT: the forward's
   const float* dlogp;     // null: 0
   const float* dentropy;  // ENT
-  __device__ bool live(int64_t r) const { return t.at(r) != t.ignore; }
+  struct Pre {
+    int64_t t;
+  };
+  struct Row {
+    Norm w;
+    float a, b;
+    int64_t t;
+  };
+  __host__ __device__ int slot_bytes() const { return sizeof(Row); }
+  __device__ Pre pre(int64_t r) const { return Pre{t.at(r)}; }
+  __device__ bool live(const Pre& p) const { return p.t != t.ignore; }
   __device__ void dead(int64_t) const {}
-  __device__ State state(int64_t r, float) const {
+  template <typename TI>
+  __device__ void prep(int64_t r, const Pre& p, const TI*, const RowIn& in, char* slot) const {
+    if ((threadIdx.x & 31) != 0) return;
+    Row& w = *reinterpret_cast<Row*>(slot);
     const float2 v = stats[r];
-    State st{v.x, v.y, 0.f};
-    if constexpr (ENT) st.u = st.s * (log2f(st.s) - entropy[r] * kLog2e);
-    return st;
+    w.w = Norm{v.x, fabsf(v.y), 0.f, !(v.y > 0.f)};
+    w.a = p.t >= 0 && p.t < in.vocab ? (dlogp ? dlogp[r] : 0.f) : __int_as_float(0x7fc00000);
+    w.b = 0.f;
+    if constexpr (ENT) {
+      w.w.u = w.w.s * (log2f(w.w.s) - entropy[r] * kLog2e);
+      w.b = dentropy[r];
+    }
+    w.t = p.t;
   }
-  template <typename TI>
-  __device__ void begin(int64_t, const TI*, int, char*) const {}
-  template <typename TI>
-  __device__ Coef finish(int64_t r, const State& st, const TI*, const RowIn& in, float g, bool, char*) const {
-    const int64_t tr = t.at(r);
-    const float a = tr >= 0 && tr < in.vocab ? (dlogp ? dlogp[r] : 0.f) : __int_as_float(0x7fc00000);
-    return coef_of(a, ENT ? dentropy[r] : 0.f, g, st, in.inv_tau);
-  }
-  template <typename TO, typename TI>
-  __device__ void fix(int64_t r, const State& st, const Coef& cf, TO* dx, int lo, int hi, const TI* x, const RowIn& in, float, char*) const {
-    fix_target<ENT>(t.at(r), st, cf, dx, lo, hi, x, in);
+  __device__ Norm state(const char* slot) const { return reinterpret_cast<const Row*>(slot)->w; }
+  __device__ Coef finish(int64_t, const Norm& w, const RowIn& in, float g, bool, char* slot) const {
+    const Row& row = *reinterpret_cast<const Row*>(slot);
+    return coef_of(row.a, row.b, g, row.t, w, in);
   }
 };
 
 // ENT: the entropy bonus takes part in the gradient (its value is always written).
 template <bool ENT>
 struct Policy {
-  static constexpr bool kEnt = true, kGradEnt = ENT, kHasStats = false;
+  static constexpr bool kEnt = true, kGradEnt = ENT, kHasStats = false, kList = false, kForwardOnly = false;
   Targets t;
   const float* old_logp;
   const float* adv;
@@ -104,41 +109,48 @@ struct Policy {
   float* entropy;
   float* kl;
   uint8_t* clipped;
-  __device__ float weight(int64_t r) const { return weights ? weights[r] : uniform; }
-  __device__ bool live(int64_t r) const { return t.at(r) != t.ignore && weight(r) != 0.f; }
+  struct Pre {
+    int64_t t;
+    float w;
+  };
+  struct Row {
+    int64_t t;
+    float w, xt, old_logp, adv, ref;
+  };
+  __host__ __device__ int slot_bytes() const { return sizeof(Row); }
+  __device__ Pre pre(int64_t r) const { return Pre{t.at(r), weights ? weights[r] : uniform}; }
+  __device__ bool live(const Pre& p) const { return p.t != t.ignore && p.w != 0.f; }
   __device__ void dead(int64_t r) const {
     terms[r] = logp[r] = entropy[r] = kl[r] = 0.f;
     clipped[r] = 0;
   }
   template <typename TI>
-  __device__ void begin(int64_t, const TI*, int, char*) const {}
-  template <typename TI>
-  __device__ Coef finish(int64_t r, const State& st, const TI* x, const RowIn& in, float g, bool writer, char*) const {
-    const float w = weight(r), a = adv[r];
-    const float lp = logp_of(logit_at(x, t.at(r), in.vocab), st, in.k), h = entropy_of(st);
-    const float ratio = expf(lp - old_logp[r]);
-    const float plain = ratio * a, bounded = fminf(fmaxf(ratio, 1.f - lo), 1.f + hi) * a;
+  __device__ void prep(int64_t r, const Pre& p, const TI* x, const RowIn& in, char* slot) const {
+    if ((threadIdx.x & 31) == 0)
+      *reinterpret_cast<Row*>(slot) = Row{p.t, p.w, logit_at(x, p.t, in.vocab), old_logp[r], adv[r], ref ? ref[r] : 0.f};
+  }
+  __device__ Coef finish(int64_t r, const Norm& w, const RowIn& in, float g, bool writer, char* slot) const {
+    const Row row = *reinterpret_cast<const Row*>(slot);
+    const float lp = logp_of(row.xt, w, in), h = entropy_of(w);
+    const float ratio = expf(lp - row.old_logp);
+    const float plain = ratio * row.adv, bounded = fminf(fmaxf(ratio, 1.f - lo), 1.f + hi) * row.adv;
     const bool cut = bounded < plain;
     float per = cut ? -bounded : -plain, da = cut ? 0.f : -plain, klv = 0.f;
     if (ref) {
-      const float d = ref[r] - lp, em = expm1f(d);
+      const float d = row.ref - lp, em = expm1f(d);
       klv = em - d;
       per = fmaf(beta, klv, per);
       da = fmaf(-beta, em, da);
     }
     per = fmaf(-ent_coef, h, per);
-    if (writer && threadIdx.x == 0) {
-      terms[r] = w * per;
+    if (writer && (threadIdx.x & 31) == 0) {
+      terms[r] = row.w * per;
       logp[r] = lp;
       entropy[r] = h;
       kl[r] = klv;
       clipped[r] = cut;
     }
-    return coef_of(w * da, ENT ? -w * ent_coef : 0.f, g, st, in.inv_tau);
-  }
-  template <typename TO, typename TI>
-  __device__ void fix(int64_t r, const State& st, const Coef& cf, TO* dx, int lo_, int hi_, const TI* x, const RowIn& in, float, char*) const {
-    fix_target<ENT>(t.at(r), st, cf, dx, lo_, hi_, x, in);
+    return coef_of(row.w * da, ENT ? -row.w * ent_coef : 0.f, g, row.t, w, in);
   }
 };
 
@@ -253,11 +265,10 @@ __global__ void __launch_bounds__(kPairThreads) pairs_kernel(Pairs a) {
     for (int64_t i = hi[1] + threadIdx.x; i < a.rows; i += blockDim.x) a.coef[i] = 0.f;
 }
 
-static RowIn row_in(const void* logits, int64_t rows, int64_t vocab, int64_t ld, float temperature) {
-  return RowIn{logits, rows, vocab, ld, kLog2e / temperature, 1.f / temperature};
-}
-
 }  // namespace rowloss
+
+FERRITE_DEFINE_STATUS_READER(status_logprobs)
+
 }  // namespace ferrite
 
 using namespace ferrite;
@@ -276,8 +287,8 @@ int ferrite_logprobs_fwd(void* stream, const void* logits, const void* targets, 
   const RowIn in = row_in(logits, rows, vocab, ld, temperature);
   const Targets t{targets, target_dtype, ignore_index};
   cudaStream_t s = (cudaStream_t)stream;
-  if (entropy) return dispatch_row(s, in, RowOut{}, LogprobsFwd<true>{t, logp, entropy, (float2*)stats}, dtype, -1, 0, op);
-  return dispatch_row(s, in, RowOut{}, LogprobsFwd<false>{t, logp, nullptr, (float2*)stats}, dtype, -1, 0, op);
+  if (entropy) return dispatch_row(s, in, RowOut{}, LogprobsFwd<true>{t, logp, entropy, (float2*)stats}, dtype, -1, op);
+  return dispatch_row(s, in, RowOut{}, LogprobsFwd<false>{t, logp, nullptr, (float2*)stats}, dtype, -1, op);
 }
 
 int ferrite_logprobs_bwd(void* stream, const void* logits, const void* targets, const float* stats, const float* entropy,
@@ -295,8 +306,8 @@ int ferrite_logprobs_bwd(void* stream, const void* logits, const void* targets, 
   const RowOut out{dlogits, ld_out, dloss, scale};
   const Targets t{targets, target_dtype, ignore_index};
   cudaStream_t s = (cudaStream_t)stream;
-  if (dentropy) return dispatch_row(s, in, out, LogprobsBwd<true>{t, (const float2*)stats, entropy, dlogp, dentropy}, dtype, out_dtype, 0, op);
-  return dispatch_row(s, in, out, LogprobsBwd<false>{t, (const float2*)stats, nullptr, dlogp, nullptr}, dtype, out_dtype, 0, op);
+  if (dentropy) return dispatch_row(s, in, out, LogprobsBwd<true>{t, (const float2*)stats, entropy, dlogp, dentropy}, dtype, out_dtype, op);
+  return dispatch_row(s, in, out, LogprobsBwd<false>{t, (const float2*)stats, nullptr, dlogp, nullptr}, dtype, out_dtype, op);
 }
 
 int ferrite_policy_loss(void* stream, const void* logits, const void* targets, const float* old_logp, const float* advantages,
@@ -323,9 +334,9 @@ int ferrite_policy_loss(void* stream, const void* logits, const void* targets, c
     const int od = dlogits ? out_dtype : -1;
     int rc;
     if (entropy_coef != 0.f && dlogits)
-      rc = dispatch_row(s, in, out, Policy<true>{t, old_logp, advantages, weights, ref_logp, clip_low, clip_high, kl_coef, entropy_coef, uniform, workspace, logp, entropy, kl, clipped}, dtype, od, 0, op);
+      rc = dispatch_row(s, in, out, Policy<true>{t, old_logp, advantages, weights, ref_logp, clip_low, clip_high, kl_coef, entropy_coef, uniform, workspace, logp, entropy, kl, clipped}, dtype, od, op);
     else
-      rc = dispatch_row(s, in, out, Policy<false>{t, old_logp, advantages, weights, ref_logp, clip_low, clip_high, kl_coef, entropy_coef, uniform, workspace, logp, entropy, kl, clipped}, dtype, od, 0, op);
+      rc = dispatch_row(s, in, out, Policy<false>{t, old_logp, advantages, weights, ref_logp, clip_low, clip_high, kl_coef, entropy_coef, uniform, workspace, logp, entropy, kl, clipped}, dtype, od, op);
     if (rc) return rc;
   }
   return sum_terms(s, workspace, loss, rows, 1.f, op);

@@ -1,141 +1,603 @@
-// The kernel that runs one row loss (an Op, see rowloss.cuh for the mathematics) over
-// logits [rows, vocab]: one CTA per row, one pass for (m, s, u), a block merge, and a
-// second pass over the same row (by then in L2) that writes the gradient.
+// The kernels that run one row loss (an Op; the mathematics is in rowloss.cuh) over logits
+// [rows, vocab].
 //
 // An Op provides
-//   kEnt        whether the sum of e * y is needed for the gradient or the entropy
-//   kHasStats   the row's state is an input (no first pass)
-//   live(r)     false: the row is masked -- it is not read, its results are zeros
-//   dead(r)     writes a masked row's results (one thread)
-//   begin(...)  what can start before the row's state is known (all threads)
-//   finish(...) the row's results from its state; returns the gradient's coefficients (all threads)
-//   fix(...)    the gradient entries that are not e (A + B y): after the row is written
+//   kEnt        the sum of e * y is needed (the entropy's value, or its gradient)
+//   kGradEnt    the gradient has the entropy's term
+//   kHasStats   the row's state is an input: no first pass
+//   kList       the gradient has more single entries than the target's
+//   Pre, pre(r), live(pre), dead(r)   masked rows: not read, results and gradient zero
+//   slot_bytes()                      shared memory of one row
+//   prep(r, pre, x, in, slot)         one warp: what does not need the row's state
+//   finish(r, norm, in, g, writer, slot)  one warp: the results, written by `writer`; returns the
+//                                       gradient's coefficients in every lane
+//   state(slot)                       kHasStats: the state that prep loaded
+//   fix(...)                          kList: the single entries, after the row is written
 #pragma once
+
+#include <atomic>
 
 #include "rowloss.cuh"
 
 namespace ferrite {
 namespace rowloss {
 
-// Calls f(i, vals) for every vector of N = 16 / sizeof(T) elements of x[0, n) whose address is
-// a multiple of 16, and g(i, x_i) for the elements before and after those, over the CTA's threads.
-template <typename T, typename F, typename G>
-__device__ __forceinline__ void for_row(const T* x, int n, F&& f, G&& g) {
-  constexpr int N = 16 / sizeof(T);
-  const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-  const int nv = (n - head) / N;
-  const int tail = head + nv * N;
-  const int tid = threadIdx.x;
-  for (int v = tid; v < nv; v += blockDim.x) {
-    const int i = head + v * N;
-    float vals[N];
-    unpack16<T>(ld_stream_v4(x + i), vals);
-    f(i, vals);
+// A row cut into 16-byte vectors: `head` elements up to the first 16-byte boundary, nv
+// vectors, and the rest.
+template <typename T>
+struct RowCut {
+  static constexpr int N = 16 / sizeof(T);
+  int n, head, nv, tail;
+  __device__ __forceinline__ RowCut(const T* x, int n_) : n(n_) {
+    head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
+    nv = (n - head) / N;
+    tail = head + nv * N;
   }
-  if (tid < head) g(tid, DT<T>::to_f(x[tid]));
-  if (tid < n - tail) g(tail + tid, DT<T>::to_f(x[tail + tid]));
+};
+// Whether N elements of dx starting at column `head` can be stored as one vector.
+template <typename TO, int N>
+__device__ __forceinline__ bool vector_rows(const TO* dx, int head) {
+  return (reinterpret_cast<uintptr_t>(dx + head) & (N * sizeof(TO) - 1)) == 0;
+}
+template <typename TO, int N>
+__device__ __forceinline__ void store_at(TO* p, const float (&d)[N], bool vec) {
+  if (vec) {
+    store_vec<TO, N>(p, d);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) p[j] = DT<TO>::from_f(d[j]);
+  }
 }
 
-template <bool ENT>
-__device__ __forceinline__ State block_merge(State st, float k, State* sh) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    State o;
-    o.m = __shfl_xor_sync(0xffffffffu, st.m, off);
-    o.s = __shfl_xor_sync(0xffffffffu, st.s, off);
-    o.u = ENT ? __shfl_xor_sync(0xffffffffu, st.u, off) : 0.f;
-    merge<ENT>(st, o, k);
-  }
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = st;
-  __syncthreads();
-  st = sh[0];
-  for (int w = 1; w < (int)(blockDim.x >> 5); ++w) merge<ENT>(st, sh[w], k);
-  return st;
-}
+// --------------------------------------------------------------------------
+// Any row: one CTA per row, which reads it twice (the second time mostly from L2).  Serves the
+// vocabularies whose row does not fit the shared memory of a cluster.
+// --------------------------------------------------------------------------
 
 template <class Op, typename TI, typename TO, bool GRAD>
 __global__ void __launch_bounds__(512) row_kernel(RowIn in, RowOut out, Op op) {
-  extern __shared__ __align__(16) char sh_op[];
+  extern __shared__ __align__(16) char slot[];
   __shared__ State sh_state[16];
+  __shared__ Coef sh_coef;
+  constexpr int N = 16 / sizeof(TI);
   pdl_launch_dependents();
   pdl_wait();
   const int64_t r = blockIdx.x;
-  const int n = (int)in.vocab;
+  const int n = (int)in.vocab, tid = threadIdx.x, nt = blockDim.x, warp = tid >> 5, lane = tid & 31;
   const TI* x = static_cast<const TI*>(in.logits) + r * in.ld;
   TO* dx = GRAD ? static_cast<TO*>(out.dlogits) + r * out.ld : nullptr;
-  if (!op.live(r)) {
-    if (threadIdx.x == 0) op.dead(r);
+  const auto pre = op.pre(r);
+  if (!op.live(pre)) {
+    if (tid == 0) op.dead(r);
     if constexpr (GRAD)
-      for (int i = threadIdx.x; i < n; i += blockDim.x) dx[i] = DT<TO>::from_f(0.f);
+      for (int i = tid; i < n; i += nt) dx[i] = DT<TO>::from_f(0.f);
     return;
   }
-  op.begin(r, x, n, sh_op);
+  const RowCut<TI> cut(x, n);
+  if (warp == 0) op.prep(r, pre, x, in, slot);
   State st = empty_state();
-  if constexpr (Op::kHasStats) {
-    st = op.state(r, in.k);
-  } else {
-    for_row<TI>(
-        x, n, [&](int, const float(&v)[16 / sizeof(TI)]) { push<Op::kEnt>(st, v, in.k); },
-        [&](int, float v) {
-          const float one[1] = {v};
-          push<Op::kEnt>(st, one, in.k);
-        });
-    st = block_merge<Op::kEnt>(st, in.k, sh_state);
+  if constexpr (!Op::kHasStats) {
+    for (int v = tid; v < cut.nv; v += nt) {
+      float vals[N];
+      unpack16<TI>(ld_stream_v4(x + cut.head + v * N), vals);
+      if (v == tid) st.m = vals[0];
+      push<Op::kEnt>(st, vals, in);
+    }
+    const int e = tid < cut.head ? tid : tid - cut.head + cut.tail;  // an element before or after the vectors
+    if (e < cut.head || (tid >= cut.head && e < n)) {
+      const float one[1] = {DT<TI>::to_f(x[e])};
+      push<Op::kEnt>(st, one, in);
+    }
+    st = warp_merge<Op::kEnt>(st, in);
+    if (lane == 0) sh_state[warp] = st;
+    __syncthreads();
   }
-  const float g = GRAD ? (out.dloss ? *out.dloss : 1.f) * out.scale : 0.f;
-  const Coef cf = op.finish(r, st, x, in, g, true, sh_op);
+  if (warp == 0) {
+    __syncwarp();
+    Norm w;
+    if constexpr (Op::kHasStats) w = op.state(slot);
+    else w = normalise<Op::kEnt>(warp_merge<Op::kEnt>(lane < (nt >> 5) ? sh_state[lane] : empty_state(), in), in);
+    const float g = GRAD ? (out.dloss ? *out.dloss : 1.f) * out.scale : 0.f;
+    const Coef cf = op.finish(r, w, in, g, true, slot);
+    if (lane == 0) sh_coef = cf;
+  }
   if constexpr (GRAD) {
+    __syncthreads();
+    const Coef cf = sh_coef;
     if (cf.masked) {
-      for (int i = threadIdx.x; i < n; i += blockDim.x) dx[i] = DT<TO>::from_f(0.f);
+      for (int i = tid; i < n; i += nt) dx[i] = DT<TO>::from_f(0.f);
       return;
     }
-    constexpr int N = 16 / sizeof(TI);
-    const float c = st.m * in.k;
-    const bool big = is_big(c);
-    const int head = (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(TI));
-    const bool vec = (reinterpret_cast<uintptr_t>(dx + head) & (N * sizeof(TO) - 1)) == 0;
-    for_row<TI>(
-        x, n,
-        [&](int i, const float(&v)[N]) {
-          float d[N];
+    const bool vec = vector_rows<TO, N>(dx, cut.head);
+    for (int v = tid; v < cut.nv; v += nt) {
+      const int i = cut.head + v * N;
+      float vals[N], d[N];
+      unpack16<TI>(ld_stream_v4(x + i), vals);
+      grads_of<Op::kGradEnt>(vals, d, i, in.k, cf);
+      store_at(dx + i, d, vec);
+    }
+    const int e = tid < cut.head ? tid : tid - cut.head + cut.tail;
+    if (e < cut.head || (tid >= cut.head && e < n))
+      dx[e] = DT<TO>::from_f(grad_of<Op::kGradEnt>(DT<TI>::to_f(x[e]), in.k, cf) + (e == cf.t ? cf.at_t : 0.f));
+    if constexpr (Op::kList) {
+      __syncthreads();  // the entries below overwrite what another thread has stored
+      op.template fix<TO>(cf, dx, 0, n, in, slot, tid, nt);
+    }
+  }
+}
+
+// --------------------------------------------------------------------------
+// Rows that fit: one read, one write.
+//
+// Bound: HBM.  A row is read once into shared memory, and both passes (the sums, then the
+// gradient) read it there; so traffic is the logits plus the gradient, and the next bound is the
+// ex2 unit (16 a clock and SM: two per element, or one without a gradient).
+//
+// A persistent cluster of C CTAs, one CTA to an SM, takes rows cluster, cluster + clusters, ...; each
+// CTA holds 1/C of a row.  C is 1 unless two such slices do not fit a CTA's shared memory.  In a CTA
+//   - one warp issues untiled bulk copies of 16 KB chunks into a ring (mbarriers full / empty), as far
+//     ahead as the ring allows;
+//   - kWarps warps run the passes: the sums of row i chunk by chunk as they land, then the gradient
+//     of row i - 1 from its resident chunks, released one by one.  One row's lag hides everything
+//     between a row's two passes;
+//   - that is the work of kHelpers warps, row i to helper i mod kHelpers: fetch what the row's loss
+//     needs besides the logits (ahead of time), merge the passes' states (and the C CTAs', through
+//     distributed shared memory, in rank order), write the row's results, hand back the gradient's
+//     coefficients, and at last write the single entries of a list.
+// Every wait is bounded; an expired one raises the CTA's abort flag and the status word, after which
+// no copy is issued, nobody waits, and the copies in flight are waited for before the CTA exits.
+// --------------------------------------------------------------------------
+
+constexpr int kWarps = 16;
+constexpr int kPass = kWarps * 32;              // threads of the passes
+constexpr int kHelpers = 6;
+constexpr int kRingThreads = kPass + 32 + kHelpers * 32;
+constexpr int kChunk = 16384;                   // bytes
+constexpr int kChunkVec = kChunk / 16;
+constexpr int kVecPer = kChunkVec / kPass;      // vectors a thread takes of a chunk
+constexpr int kMaxChunks = 14;
+constexpr int kRingCluster = 8;
+
+struct RingShared {
+  uint64_t full[kMaxChunks], empty[kMaxChunks];
+  // of a helper's row: the passes' states are there; its coefficients are; its gradient is written;
+  // the other CTAs' states are there
+  // (two places in turn: a CTA that is a whole turn of the helpers ahead must not reach into a
+  // place that another still reads)
+  uint64_t states[kHelpers], done[kHelpers], written[kHelpers], peers[kHelpers][2];
+  State warp_state[kHelpers][kWarps];
+  State peer_state[kHelpers][2][kRingCluster];
+  Coef coef[kHelpers];
+  int abort;
+};
+constexpr int kRingHeader = (int)((sizeof(RingShared) + 127) / 128 * 128);
+
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// The bounded wait of common.cuh for warps that run ahead of the passes: it sleeps between tries, so
+// that it takes no issue slots from them.  CLUSTER: other CTAs of the cluster arrive on the barrier.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait_idle(uint64_t* bar, uint32_t parity, volatile int* abort, int where) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!(CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity))) {
+    if (*abort) return false;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      report_timeout(where);
+      *abort = 1;
+      return false;
+    }
+    __nanosleep(40);
+  }
+  return true;
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// A row as one CTA of the cluster sees it: its slice of the vectors, and (first and last CTA) the
+// elements before and after them.
+template <typename T>
+struct Slice {
+  RowCut<T> cut;
+  int v0, nv, chunks;
+  bool first, last;
+  __device__ __forceinline__ Slice(const T* x, int n, int rank, int lg_cluster) : cut(x, n) {
+    const int size = 1 << lg_cluster, per = (cut.nv + size - 1) >> lg_cluster;
+    v0 = min(rank * per, cut.nv);
+    nv = min(per, cut.nv - v0);
+    chunks = (nv + kChunkVec - 1) / kChunkVec;
+    first = rank == 0;
+    last = rank == size - 1;
+  }
+  __device__ __forceinline__ int col0() const { return cut.head + v0 * RowCut<T>::N; }
+  __device__ __forceinline__ int lo() const { return first ? 0 : col0(); }
+  __device__ __forceinline__ int hi() const { return last ? cut.n : col0() + nv * RowCut<T>::N; }
+  // the column of the element outside the vectors that thread tid takes, or -1
+  __device__ __forceinline__ int edge(int tid) const {
+    if (first && tid < cut.head) return tid;
+    const int e = cut.tail + tid - 16;
+    return last && tid >= 16 && e < cut.n ? e : -1;
+  }
+};
+
+// Which of the rows r, r + step, ... are live, asked row by row by a whole warp: 32 rows' masks are
+// fetched at a time, so that a row's own is never waited for.
+template <class Op>
+struct LiveRows {
+  const Op& op;
+  int64_t rows, step;
+  uint32_t mask = 0;
+  int left = 0;
+  __device__ __forceinline__ bool next(int64_t r) {
+    if (left == 0) {
+      const int64_t q = r + (int64_t)(threadIdx.x & 31) * step;
+      mask = __ballot_sync(0xffffffffu, q < rows && op.live(op.pre(q)));
+      left = 32;
+    }
+    const bool live = mask & 1u;
+    mask >>= 1;
+    --left;
+    return live;
+  }
+};
+
+// A place in the ring, and the parity of its current use.
+struct Place {
+  int at = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next(int size) {
+    if (++at == size) {
+      at = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+template <class Op, typename TI, typename TO, bool GRAD>
+__global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut out, Op op, int ring_chunks, int lg_cluster) {
+  constexpr int N = 16 / sizeof(TI);
+  constexpr bool kSums = !Op::kHasStats;        // a first pass
+  constexpr bool kLag = GRAD && kSums;          // both passes: the second one row behind
+  constexpr bool kFix = GRAD && Op::kList;
+  extern __shared__ __align__(128) char smem[];
+  RingShared& sh = *reinterpret_cast<RingShared*>(smem);
+  char* ring = smem + kRingHeader;
+  const int slot_bytes = (op.slot_bytes() + 15) & ~15;
+  char* slots = ring + (size_t)ring_chunks * kChunk;
+  volatile int* abort = &sh.abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cluster = 1 << lg_cluster;
+  const int rank = cluster > 1 ? (int)cluster_ctarank() : 0;
+  const int n = (int)in.vocab;
+  const int64_t step = gridDim.x >> lg_cluster, r0 = blockIdx.x >> lg_cluster;
+  if (tid == 0) {
+    for (int i = 0; i < ring_chunks; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], kWarps);
+    }
+    for (int i = 0; i < kHelpers; ++i) {
+      mbar_init(&sh.states[i], kWarps);
+      mbar_init(&sh.done[i], 1);
+      mbar_init(&sh.written[i], kWarps);
+      mbar_init(&sh.peers[i][0], cluster);
+      mbar_init(&sh.peers[i][1], cluster);
+    }
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  pdl_launch_dependents();
+  __syncthreads();
+  if (cluster > 1) cluster_sync_all();  // the peers' barriers are ready
+  pdl_wait();
+
+  LiveRows<Op> rows{op, in.rows, step};
+  if (warp == kWarps) {  // ---- copies
+    Place p;
+    uint32_t issued = 0;
+    bool stop = false;
+    for (int64_t r = r0; r < in.rows; r += step) {
+      if (!rows.next(r) || lane != 0 || stop) continue;
+      const TI* x = static_cast<const TI*>(in.logits) + r * in.ld;
+      const Slice<TI> sl(x, n, rank, lg_cluster);
+      const char* src = reinterpret_cast<const char*>(x + sl.col0());
+      int left = sl.nv;
+      for (int c = 0; c < sl.chunks; ++c) {
+        if (issued >= (uint32_t)ring_chunks && !wait_idle(&sh.empty[p.at], p.parity ^ 1, abort, 201)) {
+          stop = true;
+          break;
+        }
+        const uint32_t bytes = (uint32_t)min(left, kChunkVec) * 16u;
+        mbar_arrive_expect_tx(&sh.full[p.at], bytes);
+        bulk_load(ring + (size_t)p.at * kChunk, src, bytes, &sh.full[p.at]);
+        src += bytes;
+        left -= kChunkVec;
+        p.next(ring_chunks);
+        ++issued;
+      }
+    }
+    if (lane == 0) {
+      // the last copy into each chunk has landed before the CTA gives up its shared memory
+      for (int j = 0; j < ring_chunks && (uint32_t)j < issued; ++j) {
+        if (p.at == 0) p.parity ^= 1;
+        p.at = (p.at == 0 ? ring_chunks : p.at) - 1;
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(&sh.full[p.at], p.parity))
+          if (globaltimer_ns() - t0 > kWaitLimitNs) {
+            report_timeout(202);
+            *abort = 1;
+            break;
+          }
+      }
+    }
+  } else if (warp > kWarps) {  // ---- what lies between a row's two passes
+    const int h = warp - kWarps - 1;
+    char* slot = slots + h * slot_bytes;
+    const float g = GRAD ? (out.dloss ? *out.dloss : 1.f) * out.scale : 0.f;
+    int turn = 0;
+    uint32_t parity = 0, half = 0, half_parity = 0;  // of this helper's barriers; which of the two peers' places
+    for (int64_t r = r0; r < in.rows; r += step) {
+      if (!rows.next(r)) continue;
+      const bool my_turn = turn == h;
+      if (++turn == kHelpers) turn = 0;
+      if (!my_turn) continue;
+      const TI* x = static_cast<const TI*>(in.logits) + r * in.ld;
+      op.prep(r, op.pre(r), x, in, slot);
+      __syncwarp();
+      Norm w;
+      if constexpr (kSums) {
+        (void)wait_idle(&sh.states[h], parity, abort, 203);
+        __syncwarp();
+        State st = warp_merge<Op::kEnt>(lane < kWarps ? sh.warp_state[h][lane] : empty_state(), in);
+        if (cluster > 1) {
+          if (lane < cluster) {
+            const uint32_t to = mapa_shared(&sh.peer_state[h][half][rank], lane);
+            st_cluster(to, st.m);
+            st_cluster(to + 4, st.s);
+            st_cluster(to + 8, st.u);
+            mbar_arrive_cluster(mapa_shared(&sh.peers[h][half], lane));
+          }
+          (void)wait_idle<true>(&sh.peers[h][half], half_parity, abort, 204);
+          __syncwarp();
+          st = warp_merge<Op::kEnt>(lane < cluster ? sh.peer_state[h][half][lane] : empty_state(), in);
+          half_parity ^= half;
+          half ^= 1;
+        }
+        w = normalise<Op::kEnt>(st, in);
+      } else {
+        w = op.state(slot);
+      }
+      const Coef cf = op.finish(r, w, in, g, rank == 0, slot);
+      if constexpr (!kSums) {
+        // the passes have read the coefficients of the row before in this place
+        (void)wait_idle(&sh.written[h], parity ^ 1, abort, 205);
+        __syncwarp();
+      }
+      if (lane == 0) {
+        sh.coef[h] = cf;
+        mbar_arrive(&sh.done[h]);
+      }
+      if constexpr (kFix) {
+        (void)wait_idle(&sh.written[h], parity, abort, 206);
+        __syncwarp();
+        if (!cf.masked) {
+          const Slice<TI> sl(x, n, rank, lg_cluster);
+          op.template fix<TO>(cf, static_cast<TO*>(out.dlogits) + r * out.ld, sl.lo(), sl.hi(), in, slot, lane, 32);
+        }
+        __syncwarp();
+      }
+      parity ^= 1;
+    }
+  } else {  // ---- the passes
+    Place p1, p2, slot1, slot2;  // chunks and helpers of the first and the second pass
+    // the second pass of row r: its gradient, from the chunks at p2
+    auto second = [&](int64_t r) {
+      const TI* x = static_cast<const TI*>(in.logits) + r * in.ld;
+      TO* dx = static_cast<TO*>(out.dlogits) + r * out.ld;
+      const Slice<TI> sl(x, n, rank, lg_cluster);
+      const int col0 = sl.col0(), edge = sl.edge(tid);
+      const bool vec = vector_rows<TO, N>(dx, sl.cut.head);
+      const float edge_x = edge >= 0 ? DT<TI>::to_f(x[edge]) : 0.f;
+      (void)mbar_wait(&sh.done[slot2.at], slot2.parity, abort, 207);
+      const Coef cf = sh.coef[slot2.at];
+      int left = sl.nv - tid;
+      TO* to = dx + col0 + tid * N;
+      for (int c = 0; c < sl.chunks; ++c) {
+        if constexpr (!kSums) (void)mbar_wait(&sh.full[p2.at], p2.parity, abort, 208);
+        const uint4* p = reinterpret_cast<const uint4*>(ring + (size_t)p2.at * kChunk) + tid;
+        uint4 raw[kVecPer];
 #pragma unroll
-          for (int j = 0; j < N; ++j) d[j] = grad_of<Op::kGradEnt>(v[j], in.k, st.m, c, big, cf.A, cf.B);
-          if (vec) {
-            store_vec<TO, N>(dx + i, d);
+        for (int q = 0; q < kVecPer; ++q)
+          if (q * kPass < left) raw[q] = p[q * kPass];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.empty[p2.at]);
+        p2.next(ring_chunks);
+#pragma unroll
+        for (int q = 0; q < kVecPer; ++q)
+          if (q * kPass < left) {
+            float vals[N], d[N] = {};
+            unpack16<TI>(raw[q], vals);
+            if (!cf.masked) grads_of<Op::kGradEnt>(vals, d, (int)(to - dx) + q * kPass * N, in.k, cf);
+            store_at(to + q * kPass * N, d, vec);
+          }
+        left -= kChunkVec;
+        to += kChunkVec * N;
+      }
+      if (edge >= 0)
+        dx[edge] = DT<TO>::from_f(cf.masked ? 0.f : grad_of<Op::kGradEnt>(edge_x, in.k, cf) + (edge == cf.t ? cf.at_t : 0.f));
+      if constexpr (kFix || !kSums) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.written[slot2.at]);
+      }
+      slot2.next(kHelpers);
+    };
+    int64_t last = -1;  // kLag: the row whose second pass is due
+    for (int64_t r = r0; r < in.rows; r += step) {
+      if (!rows.next(r)) {
+        if (tid == 0 && rank == 0) op.dead(r);
+        if constexpr (GRAD) {
+          TO* dx = static_cast<TO*>(out.dlogits) + r * out.ld;
+          const Slice<TI> sl(static_cast<const TI*>(in.logits) + r * in.ld, n, rank, lg_cluster);
+          const bool vec = vector_rows<TO, N>(dx, sl.cut.head);
+          const float zero[N] = {};
+          for (int v = tid; v < sl.nv; v += kPass) store_at(dx + sl.col0() + v * N, zero, vec);
+          const int edge = sl.edge(tid);
+          if (edge >= 0) dx[edge] = DT<TO>::from_f(0.f);
+        }
+        continue;
+      }
+      if constexpr (kSums) {
+        const TI* x = static_cast<const TI*>(in.logits) + r * in.ld;
+        const Slice<TI> sl(x, n, rank, lg_cluster);
+        const int edge = sl.edge(tid);
+        const float edge_x = edge >= 0 ? DT<TI>::to_f(x[edge]) : 0.f;
+        State st = empty_state();
+        int left = sl.nv - tid;
+        for (int c = 0; c < sl.chunks; ++c) {
+          (void)mbar_wait(&sh.full[p1.at], p1.parity, abort, 209);
+          const uint4* p = reinterpret_cast<const uint4*>(ring + (size_t)p1.at * kChunk) + tid;
+          if ((kVecPer - 1) * kPass < left) {
+            float vals[N * kVecPer];
+#pragma unroll
+            for (int q = 0; q < kVecPer; ++q) unpack16<TI>(p[q * kPass], *reinterpret_cast<float(*)[N]>(&vals[q * N]));
+            if (c == 0) st.m = vals[0];
+            push<Op::kEnt>(st, vals, in);
           } else {
 #pragma unroll
-            for (int j = 0; j < N; ++j) dx[i + j] = DT<TO>::from_f(d[j]);
+            for (int q = 0; q < kVecPer - 1; ++q)
+              if (q * kPass < left) {
+                float vals[N];
+                unpack16<TI>(p[q * kPass], vals);
+                if (c == 0 && q == 0) st.m = vals[0];
+                push<Op::kEnt>(st, vals, in);
+              }
           }
-        },
-        [&](int i, float v) { dx[i] = DT<TO>::from_f(grad_of<Op::kGradEnt>(v, in.k, st.m, c, big, cf.A, cf.B)); });
-    __syncthreads();  // the entries below overwrite what another thread has stored
-    op.template fix<TO>(r, st, cf, dx, 0, n, x, in, g, sh_op);
+          if constexpr (!kLag) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.empty[p1.at]);
+          }
+          p1.next(ring_chunks);
+          left -= kChunkVec;
+        }
+        if (edge >= 0) {
+          const float one[1] = {edge_x};
+          push<Op::kEnt>(st, one, in);
+        }
+        __syncwarp();
+        st = warp_merge<Op::kEnt>(st, in);
+        // without a gradient nothing else holds the passes back until the helper has read the
+        // states of the row before in this place
+        if constexpr (!kLag) (void)mbar_wait(&sh.done[slot1.at], slot1.parity ^ 1, abort, 210);
+        if (lane == 0) {
+          sh.warp_state[slot1.at][warp] = st;
+          mbar_arrive(&sh.states[slot1.at]);
+        }
+        slot1.next(kHelpers);
+        if constexpr (kLag) {
+          if (last >= 0) second(last);
+          last = r;
+        }
+      } else {
+        second(r);
+      }
+    }
+    if constexpr (kLag)
+      if (last >= 0) second(last);
   }
+  __syncwarp();
+  if (cluster > 1) cluster_sync_all();  // nobody leaves while a peer may still write here
+}
+
+// --------------------------------------------------------------------------
+// host
+// --------------------------------------------------------------------------
+
+constexpr int kRingSmem = 227 * 1024;  // all that a CTA can have
+constexpr int kMaxSlots = kHelpers * (64 + 12 * 1024);  // the helpers' lists at their longest
+
+// How rows are split: chunks of each CTA's ring, log2 of the CTAs per row (-1: the row does not fit).
+// The split goes by the row's length and type alone, not by how many rows there are, with a gradient
+// or without: so a row's results have the same bits in every call (log-probabilities taken in one
+// batch and compared in another differ by nothing), as long as it starts on a 16-byte boundary.
+struct RingPlan {
+  int chunks, lg_cluster;
+  size_t smem;
+};
+inline RingPlan plan_ring(int64_t vocab, int elem, int slot_bytes) {
+  RingPlan p{};
+  const int slots = kHelpers * ((slot_bytes + 15) & ~15);
+  p.chunks = (kRingSmem - kRingHeader - slots) / kChunk;
+  if (p.chunks > kMaxChunks) p.chunks = kMaxChunks;
+  p.smem = (size_t)kRingHeader + (size_t)p.chunks * kChunk + slots;
+  // two slices are resident, beside lists of up to 1024 entries, and a chunk of the next
+  const int64_t most = (int64_t)(((kRingSmem - kRingHeader - kMaxSlots) / kChunk - 1) / 2) * kChunk;
+  const int64_t bytes = vocab * elem;
+  int lg = 0;
+  while ((1 << lg) < kRingCluster && ((bytes + 15) >> lg) + 16 > most) ++lg;
+  p.lg_cluster = ((bytes + 15) >> lg) + 16 > most ? -1 : lg;
+  return p;
 }
 
 inline int row_threads(int64_t vocab) { return vocab <= 1024 ? 64 : vocab <= 4096 ? 128 : vocab <= 16384 ? 256 : 512; }
 
 template <class Op, typename TI, typename TO, bool GRAD>
-static int launch_row(cudaStream_t s, const RowIn& in, const RowOut& out, const Op& op, size_t smem, const char* name) {
-  const cudaError_t e = launch_pdl(row_kernel<Op, TI, TO, GRAD>, dim3((unsigned)in.rows), dim3(row_threads(in.vocab)), smem, s, in, out, op);
+static int launch_row(cudaStream_t s, const RowIn& in, const RowOut& out, const Op& op, const char* name) {
+  const int dev = current_device();
+  if (dev < 0 || dev >= 64) return fail(FERRITE_LAUNCH_FAILED, "%s: device ordinal %d", name, dev);
+  cudaError_t e;
+  const RingPlan p = plan_ring(in.vocab, sizeof(TI), op.slot_bytes());
+  if (in.vocab * (int64_t)sizeof(TI) >= 8192 && p.lg_cluster >= 0) {
+    auto kern = ring_kernel<Op, TI, TO, GRAD>;
+    // clusters of each size that are resident at once, per device (set once; racing first calls
+    // store the same values): a persistent grid of more would run its last ones after the others
+    static std::atomic<int> resident[64][4];
+    int clusters = resident[dev][p.lg_cluster].load(std::memory_order_relaxed);
+    if (clusters == 0) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
+      if (e != cudaSuccess) return fail(FERRITE_LAUNCH_FAILED, "%s: shared memory attribute: %s", name, cudaGetErrorString(e));
+      clusters = max_active_clusters((const void*)kern, dim3(kRingThreads), kRingSmem, 1u << p.lg_cluster);
+      if (clusters < 1) clusters = 1;
+      resident[dev][p.lg_cluster].store(clusters, std::memory_order_relaxed);
+    }
+    const int64_t used = in.rows < clusters ? in.rows : clusters;
+    e = launch_pdl_cluster(kern, dim3((unsigned)(used << p.lg_cluster)), dim3(kRingThreads), p.smem, s, 1u << p.lg_cluster, in, out, op,
+                           p.chunks, p.lg_cluster);
+  } else {
+    e = launch_pdl(row_kernel<Op, TI, TO, GRAD>, dim3((unsigned)in.rows), dim3(row_threads(in.vocab)), op.slot_bytes(), s, in, out, op);
+  }
   if (e != cudaSuccess) return fail(FERRITE_LAUNCH_FAILED, "%s: %s", name, cudaGetErrorString(e));
   return check_launch(name);
 }
 
 // Dispatch on the logits' and the gradient's type (out_dtype < 0: forward only).
 template <class Op>
-static int dispatch_row(cudaStream_t s, const RowIn& in, const RowOut& out, const Op& op, int dtype, int out_dtype, size_t smem,
-                        const char* name) {
+static int dispatch_row(cudaStream_t s, const RowIn& in, const RowOut& out, const Op& op, int dtype, int out_dtype, const char* name) {
   if (out_dtype < 0) {
-    if (dtype == FERRITE_F32) return launch_row<Op, float, float, false>(s, in, out, op, smem, name);
-    if (dtype == FERRITE_BF16) return launch_row<Op, __nv_bfloat16, __nv_bfloat16, false>(s, in, out, op, smem, name);
-    return launch_row<Op, __half, __half, false>(s, in, out, op, smem, name);
+    if constexpr (Op::kHasStats) {
+      return fail(FERRITE_BAD_SHAPE, "%s: no gradient asked for", name);
+    } else {
+      if (dtype == FERRITE_F32) return launch_row<Op, float, float, false>(s, in, out, op, name);
+      if (dtype == FERRITE_BF16) return launch_row<Op, __nv_bfloat16, __nv_bfloat16, false>(s, in, out, op, name);
+      return launch_row<Op, __half, __half, false>(s, in, out, op, name);
+    }
   }
-  if (dtype == FERRITE_BF16) return launch_row<Op, __nv_bfloat16, __nv_bfloat16, true>(s, in, out, op, smem, name);
-  if (dtype == FERRITE_F16) return launch_row<Op, __half, __half, true>(s, in, out, op, smem, name);
-  if (out_dtype == FERRITE_F32) return launch_row<Op, float, float, true>(s, in, out, op, smem, name);
-  if (out_dtype == FERRITE_BF16) return launch_row<Op, float, __nv_bfloat16, true>(s, in, out, op, smem, name);
-  return launch_row<Op, float, __half, true>(s, in, out, op, smem, name);
+  if constexpr (Op::kForwardOnly) {
+    return fail(FERRITE_BAD_SHAPE, "%s: no gradient to write", name);
+  } else {
+    if (dtype == FERRITE_BF16) return launch_row<Op, __nv_bfloat16, __nv_bfloat16, true>(s, in, out, op, name);
+    if (dtype == FERRITE_F16) return launch_row<Op, __half, __half, true>(s, in, out, op, name);
+    if (out_dtype == FERRITE_F32) return launch_row<Op, float, float, true>(s, in, out, op, name);
+    if (out_dtype == FERRITE_BF16) return launch_row<Op, float, __nv_bfloat16, true>(s, in, out, op, name);
+    return launch_row<Op, float, __half, true>(s, in, out, op, name);
+  }
 }
 
 }  // namespace rowloss

@@ -6,13 +6,19 @@
 // target's, or the teacher's listed tokens), where in units of log 2
 //   k = log2(e) / tau,  y_i = k (x_i - m),  e_i = 2^y_i,  s = sum e_i,  u = sum e_i y_i,
 //   logp_i = ln2 (y_i - log2 s),   H = ln2 (log2 s - u / s),   p_i = e_i / s.
-// A row's state is (m, s, u): it is built in one pass (running maximum, rescaled sums)
-// and merged pairwise.  All of it is f32; only the gradient is rounded, once, on store.
+// A row's state is (m, s, u): it is built in one pass and merged pairwise.  m is a base, not the
+// maximum: 2^y keeps its precision over the whole exponent range, so the first element a thread
+// sees serves, and the sums are checked instead -- a sum that reaches 2^80 (an element 2^80 above the
+// base) is redone against the largest element.  No maximum is taken per element, and no rescaling
+// runs in the usual case.  All of it is f32; only the gradient is rounded, once, on store.
 //
-// y_i is one fma(x_i, k, -c) with c = k m rounded: the same c enters every term of s
-// and of logp, so its rounding cancels.  Where k m leaves f32 (a row whose maximum is
-// the type's lowest value, or infinite) y_i is k (x_i - m) instead.  A logit of -inf
-// has e_i = 0 and contributes nothing; NaN and +inf make the row's results NaN.
+// y_i is K x_i - c with c = k m rounded -- one number for every term of s and for logp, so that its
+// rounding cancels -- and K = k + k_lo carried to twice f32: the rounding of k alone would shift
+// every log-probability the same way, and sums over long sequences would show it.  Where |c| passes
+// 2^16 (logits in the tens of thousands, rows of the type's lowest value, infinities) y_i is
+// k (x_i - m) with m the maximum.  At its end a row is normalised: c takes up log2 s, so that s is
+// 1 but for rounding and log p = ln2 y loses nothing to cancellation.  A logit of -inf has e_i = 0
+// and contributes nothing; NaN and +inf make the row's results NaN.
 #pragma once
 
 #include <cmath>
@@ -25,9 +31,10 @@ namespace rowloss {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kBig = 1e38f;  // |k m| above this: the fma form could overflow
+constexpr float kBig = 65536.f;   // |k m| above this: y is k (x - m)
+constexpr float kHuge = 0x1p80f;  // a sum above this is redone against the maximum
 
-// (m, s, u): the maximum, sum of e and sum of e * y of the elements seen so far.
+// (m, s, u): the base, sum of e and sum of e * y of the elements seen so far.
 struct State {
   float m, s, u;
 };
@@ -37,7 +44,7 @@ __device__ __forceinline__ State empty_state() { return State{-INFINITY, 0.f, 0.
 struct RowIn {
   const void* logits;
   int64_t rows, vocab, ld;
-  float k;        // log2(e) / tau
+  float k, k_lo;  // log2(e) / tau, and what its rounding left
   float inv_tau;  // 1 / tau
 };
 struct RowOut {
@@ -57,69 +64,110 @@ struct Targets {
 
 __device__ __forceinline__ bool is_big(float c) { return !(fabsf(c) <= kBig); }
 
-// y of one element against maximum m (c = k m).
-__device__ __forceinline__ float y_of(float x, float k, float m, float c) {
-  return is_big(c) ? (x - m) * k : fmaf(x, k, -c);
+// y of base m1 against base m2 >= m1 (neither -inf): the log2 of the factor that takes sums over
+// to the new base.
+__device__ __forceinline__ float base_step(float m1, float m2, const RowIn& in) {
+  const float c1 = m1 * in.k, c2 = m2 * in.k;
+  if (!is_big(c1)) return !is_big(c2) ? c1 - c2 : -(fmaf(m2, in.k, -c1) + m2 * in.k_lo);
+  return !is_big(c2) ? fmaf(m1, in.k, -c2) + m1 * in.k_lo : (m1 - m2) * in.k;
 }
 
-// Distance in y from base m1 to base m2 (<= 0 for m1 <= m2), by the same forms.
-__device__ __forceinline__ float base_step(float m1, float m2, float k) {
-  const float c1 = m1 * k, c2 = m2 * k;
-  return is_big(c1) || is_big(c2) ? (m1 - m2) * k : c1 - c2;
-}
-
+// A state's sums against base m >= st.m.  (A base of -inf means no element, or -inf and NaN only: s is 0 or NaN.)
 template <bool ENT>
-__device__ __forceinline__ void merge(State& a, const State& b, float k) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) {  // nothing but -inf on both sides (s is 0, or NaN)
-    a.s += b.s;
+__device__ __forceinline__ void rebase(State& st, float m, const RowIn& in) {
+  if (st.m == m || st.m == -INFINITY) {
+    st.m = m;
     return;
   }
-  const float da = base_step(a.m, m, k), db = base_step(b.m, m, k);
-  const float fa = ex2_approx(da), fb = ex2_approx(db);
-  if constexpr (ENT)
-    a.u = (fa > 0.f ? fa * fmaf(a.s, da, a.u) : 0.f) + (fb > 0.f ? fb * fmaf(b.s, db, b.u) : 0.f);
-  a.s = fa * a.s + fb * b.s;
-  a.m = m;
+  const float d = base_step(st.m, m, in), f = ex2_approx(d);
+  if constexpr (ENT) st.u = f > 0.f && st.s != 0.f ? f * fmaf(st.s, d, st.u) : 0.f;
+  st.s *= f;
+  st.m = m;
 }
 
-// Adds N elements to a state.
+// The states of a warp's lanes merged, in all lanes: one base, one rescaling per lane, plain sums.
+template <bool ENT>
+__device__ __forceinline__ State warp_merge(State st, const RowIn& in) {
+  float m = st.m;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  rebase<ENT>(st, m, in);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    st.s += __shfl_xor_sync(0xffffffffu, st.s, off);
+    if constexpr (ENT) st.u += __shfl_xor_sync(0xffffffffu, st.u, off);
+  }
+  return st;
+}
+
+// Adds N elements to a state: any values, against their maximum where it is above the base.
 template <bool ENT, int N>
-__device__ __forceinline__ void push(State& st, const float (&x)[N], float k) {
+__device__ __forceinline__ void push_any(State& st, const float (&x)[N], const RowIn& in) {
   float cm = x[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) cm = fmaxf(cm, x[i]);
-  if (cm > st.m) {
-    const float d = base_step(st.m, cm, k), f = ex2_approx(d);
-    if constexpr (ENT) st.u = f > 0.f ? f * fmaf(st.s, d, st.u) : 0.f;
-    st.s *= f;
-    st.m = cm;
-  }
-  const float c = st.m * k;
-  if (is_big(c)) {  // rare: see the top of the file
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (st.m == -INFINITY) {
-        if (x[i] != x[i]) st.s = x[i];
-      } else {
-        const float y = (x[i] - st.m) * k, e = ex2_approx(y);
-        st.s += e;
-        if constexpr (ENT) st.u += e > 0.f ? e * y : 0.f;
-      }
-    }
-    return;
-  }
-  float s = 0.f, u = 0.f;
+  if (cm > st.m) rebase<ENT>(st, cm, in);
+  const float c = st.m * in.k;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    float y = fmaf(x[i], k, -c);
-    const float e = ex2_approx(y);
-    s += e;
-    if constexpr (ENT) u = fmaf(e, fmaxf(y, -1000.f), u);  // y = -inf has e = 0: keep 0 * y finite
+    if (st.m == -INFINITY) {  // nothing but -inf so far
+      if (x[i] != x[i]) st.s = x[i];
+    } else {
+      const float y = is_big(c) ? (x[i] - st.m) * in.k : fmaf(x[i], in.k_lo, fmaf(x[i], in.k, -c));
+      const float e = ex2_approx(y);
+      st.s += e;
+      if constexpr (ENT) st.u += e > 0.f ? e * y : 0.f;
+    }
   }
-  st.s += s;
-  if constexpr (ENT) st.u += u;
 }
+
+// The same for the usual values: per pair of elements two packed fma (y), two ex2 and packed sums.
+template <bool ENT, int N>
+__device__ __forceinline__ void push(State& st, const float (&x)[N], const RowIn& in) {
+  if constexpr (N % 2 == 0) {
+    const float c = st.m * in.k;
+    const uint64_t k2 = f2_make(in.k, in.k), l2 = f2_make(in.k_lo, in.k_lo), c2 = f2_make(-c, -c);
+    uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const uint64_t x2 = f2_make(x[i], x[i + 1]);
+      const uint64_t y2 = f2_fma(x2, l2, f2_fma(x2, k2, c2));
+      const uint64_t e2 = f2_make(ex2_approx(f2_lo(y2)), ex2_approx(f2_hi(y2)));
+      s2 = f2_add(s2, e2);
+      if constexpr (ENT) u2 = f2_fma(e2, y2, u2);  // -inf: 0 * -inf = NaN, redone below
+    }
+    const float s = f2_lo(s2) + f2_hi(s2), u = ENT ? f2_lo(u2) + f2_hi(u2) : 0.f;
+    if (!is_big(c) && s < kHuge && (!ENT || fabsf(u) < kHuge * 128.f)) {
+      st.s += s;
+      if constexpr (ENT) st.u += u;
+      return;
+    }
+  }
+  push_any<ENT>(st, x, in);
+}
+
+// A finished row: base (c, or m where big), s, u.
+struct Norm {
+  float base, s, u;
+  int big;
+};
+// Moves the power of two of s into the base, exactly: c2 = c + j is rounded, and what the rounding
+// left goes back into s (2^err by its series: |err| <= 2^-7).
+template <bool ENT>
+__device__ __forceinline__ Norm normalise(const State& st, const RowIn& in) {
+  const float c = st.m * in.k;
+  if (is_big(c) || !(st.s < INFINITY)) return Norm{is_big(c) ? st.m : c, st.s, st.u, is_big(c)};
+  const uint32_t bits = __float_as_uint(st.s);
+  const float l = (float)((int)(bits >> 23) - 127), f = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);  // s = 2^l f
+  const float c2 = c + l, b = c2 - c, err = (c - (c2 - b)) + (l - b);  // c + l = c2 + err
+  const float t = err * kLn2, s = fmaf(f, fmaf(0.5f * t, t, t), f);
+  return Norm{c2, s, ENT ? s * (st.u / st.s - l + err) : 0.f, 0};
+}
+__device__ __forceinline__ float y_of(float x, const Norm& w, const RowIn& in) {
+  return w.big ? (x - w.base) * in.k : fmaf(x, in.k_lo, fmaf(x, in.k, -w.base));
+}
+__device__ __forceinline__ float logp_of(float xt, const Norm& w, const RowIn& in) { return (y_of(xt, w, in) - log2f(w.s)) * kLn2; }
+__device__ __forceinline__ float entropy_of(const Norm& w) { return (log2f(w.s) - w.u / w.s) * kLn2; }
 
 // 16 bytes of T as floats.
 template <typename T>
@@ -160,30 +208,71 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[N]) {
   }
 }
 
-// Gradient of one element: e (A + B y).
-template <bool ENT>
-__device__ __forceinline__ float grad_of(float x, float k, float m, float c, bool big, float A, float B) {
-  const float y = big ? (x - m) * k : fmaf(x, k, -c);
-  const float e = ex2_approx(y);
-  if constexpr (ENT) return e * fmaf(B, fmaxf(y, -1000.f), A);
-  return e * A;
-}
-
-// What the losses of one row hand to its gradient.
+// What the losses of one row hand to its gradient: dx_i = e_i (A + B y_i), and at_t more at i = t,
+// with y_i = k x_i - base, or k (x_i - base) where big.
 struct Coef {
-  float A, B;    // dx_i = e_i (A + B y_i)
-  float at_t;    // added at the target
-  bool masked;   // the row turned out to be masked: zeros
+  float base, A, B;
+  float at_t;
+  int t;            // no single entry: negative
+  int16_t big;
+  int16_t masked;   // the row turned out to be masked: zeros
 };
 
-// A, B and at_t for dL/dlogp = a and dL/dH = b: dx = g / tau (a ([i = t] - p_i) - b p_i (log p_i + H)).
-__device__ __forceinline__ Coef coef_of(float a, float b, float g, const State& st, float inv_tau) {
-  const float f = g * inv_tau;
+// Gradient of one element without the single entry.
+template <bool ENT>
+__device__ __forceinline__ float grad_of(float x, float k, const Coef& cf) {
+  const float y = cf.big ? (x - cf.base) * k : fmaf(x, k, -cf.base);
+  const float e = ex2_approx(y);
+  if constexpr (ENT) return e * fmaf(cf.B, fmaxf(y, -1000.f), cf.A);
+  return e * cf.A;
+}
+
+// Gradients of the N (even) elements x[0, N) at columns i, i + 1, ...
+template <bool ENT, int N>
+__device__ __forceinline__ void grads_of(const float (&x)[N], float (&d)[N], int i, float k, const Coef& cf) {
+  if (cf.big) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) d[j] = grad_of<ENT>(x[j], k, cf);
+  } else {
+    const uint64_t k2 = f2_make(k, k), c2 = f2_make(-cf.base, -cf.base), A2 = f2_make(cf.A, cf.A), B2 = f2_make(cf.B, cf.B);
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const uint64_t y2 = f2_fma(f2_make(x[j], x[j + 1]), k2, c2);
+      const uint64_t e2 = f2_make(ex2_approx(f2_lo(y2)), ex2_approx(f2_hi(y2)));
+      uint64_t g2 = A2;
+      if constexpr (ENT) g2 = f2_fma(B2, f2_make(fmaxf(f2_lo(y2), -1000.f), fmaxf(f2_hi(y2), -1000.f)), A2);
+      g2 = f2_mul(e2, g2);
+      d[j] = f2_lo(g2);
+      d[j + 1] = f2_hi(g2);
+    }
+  }
+  if ((unsigned)(cf.t - i) < (unsigned)N) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i + j == cf.t) d[j] += cf.at_t;
+  }
+}
+
+// The base and common factor of the gradient's y, which leaves k_lo out: k_lo x is taken at the
+// logit whose y is 0, x = base / k, where p is largest; the factor takes up the base's rounding.
+__device__ __forceinline__ float grad_base(const Norm& w, const RowIn& in, Coef& c) {
+  c.big = (int16_t)w.big;
+  c.base = w.base;
+  if (w.big) return 1.f;
+  const float shift = w.base / in.k * in.k_lo;
+  c.base = w.base - shift;
+  return ex2_approx((c.base - w.base) + shift);
+}
+// The coefficients for dL/dlogp = a and dL/dH = b: dx = g / tau (a ([i = t] - p_i) - b p_i (log p_i + H)).
+__device__ __forceinline__ Coef coef_of(float a, float b, float g, int64_t t, const Norm& w, const RowIn& in) {
+  const float f = g * in.inv_tau;
   Coef c;
+  const float scale = grad_base(w, in, c) / w.s;
+  c.t = t >= 0 && t < in.vocab ? (int)t : -1;
   c.at_t = a * f;
-  c.B = -b * f * kLn2 / st.s;
-  c.A = -a * f / st.s - c.B * (st.u / st.s);
-  c.masked = false;
+  c.B = -b * f * kLn2 * scale;
+  c.A = -a * f * scale - c.B * (w.u / w.s);
+  c.masked = 0;
   return c;
 }
 
@@ -191,6 +280,11 @@ __device__ __forceinline__ Coef coef_of(float a, float b, float g, const State& 
 // host
 // --------------------------------------------------------------------------
 inline int elem_bytes(int dtype) { return dtype == FERRITE_F32 ? 4 : 2; }
+
+inline RowIn row_in(const void* logits, int64_t rows, int64_t vocab, int64_t ld, float temperature) {
+  const double k = 1.4426950408889634 / (double)temperature;
+  return RowIn{logits, rows, vocab, ld, (float)k, (float)(k - (double)(float)k), (float)(1.0 / (double)temperature)};
+}
 
 // Sizes and types every entry point takes; `out_dtype` < 0 where there is no gradient.
 inline int check_rows(const char* op, int64_t rows, int64_t vocab, int64_t ld, float temperature, int dtype,

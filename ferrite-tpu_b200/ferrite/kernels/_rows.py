@@ -33,6 +33,19 @@ def row_stride(logits: torch.Tensor) -> int:
     return logits.stride(0) if logits.shape[0] > 1 else max(logits.stride(0), logits.shape[1])
 
 
+def empty_grad(logits: torch.Tensor, dtype) -> torch.Tensor:
+    """An uninitialised ``[rows, vocab]`` gradient, its rows apart and aligned as the logits' are (so
+    that a kernel can move both in the same vectors); dense where the logits' rows lie far apart."""
+    rows, vocab = logits.shape
+    ld = row_stride(logits)
+    if ld > vocab + max(64, vocab // 16):
+        ld = vocab
+    lead = logits.data_ptr() % 16 // logits.element_size()
+    if ld == vocab and not lead:
+        return torch.empty((rows, vocab), dtype=dtype, device=logits.device)
+    return torch.empty(rows * ld + lead, dtype=dtype, device=logits.device).as_strided((rows, vocab), (ld, 1), lead)
+
+
 def check_targets(targets: torch.Tensor, rows: int) -> tuple[torch.Tensor, int]:
     """(targets as one dense row, their type's code): int32 or int64, one for each row of logits."""
     if targets.dtype not in (torch.int32, torch.int64):

@@ -47,12 +47,12 @@ def _launch(logits, values, indices, weights, temperature, grad_dtype, dloss, gr
     top, dev = values.shape[1], logits.device
     f = torch.empty(2 * rows + 1, dtype=torch.float32, device=dev)  # loss, per-token losses and the terms of the sum
     base = f.data_ptr()
-    grad = None if grad_dtype is None else torch.empty((rows, vocab), dtype=grad_dtype, device=dev)
+    grad = None if grad_dtype is None else _rows.empty_grad(logits, grad_dtype)
     nat.check(
         nat.lib().ferrite_distill_loss(
             nat.stream_ptr(dev), logits.data_ptr(), values.data_ptr(), indices.data_ptr(), nat.ptr(weights), temperature, nat.ptr(dloss),
-            grad_scale, base, base + 4, nat.ptr(grad), base + 4 * (1 + rows), 4 * rows, rows, vocab, top, _rows.row_stride(logits), vocab,
-            top, nat.dtype_code(logits.dtype), nat.dtype_code(values.dtype), int(indices.dtype == torch.int64),
+            grad_scale, base, base + 4, nat.ptr(grad), base + 4 * (1 + rows), 4 * rows, rows, vocab, top, _rows.row_stride(logits),
+            vocab if grad is None else _rows.row_stride(grad), top, nat.dtype_code(logits.dtype), nat.dtype_code(values.dtype), int(indices.dtype == torch.int64),
             -1 if grad_dtype is None else nat.dtype_code(grad_dtype),
         )
     )

@@ -37,11 +37,11 @@ def logprobs_forward(logits, targets, temperature: float, ignore_index: int, *, 
 def logprobs_backward(logits, targets, stats, entropy, dlogp, dentropy, dloss, scale: float, temperature: float, ignore_index: int, out_dtype):
     """The gradient of ``sum(dlogp * logp + dentropy * H) * dloss * scale`` through ``ferrite_logprobs_bwd``."""
     rows, vocab = logits.shape
-    out = torch.empty((rows, vocab), dtype=out_dtype, device=logits.device)
+    out = _rows.empty_grad(logits, out_dtype)
     nat.check(
         nat.lib().ferrite_logprobs_bwd(
             nat.stream_ptr(logits.device), logits.data_ptr(), targets.data_ptr(), stats.data_ptr(), nat.ptr(entropy), nat.ptr(dlogp),
-            nat.ptr(dentropy), nat.ptr(dloss), scale, out.data_ptr(), rows, vocab, _rows.row_stride(logits), vocab, ignore_index,
+            nat.ptr(dentropy), nat.ptr(dloss), scale, out.data_ptr(), rows, vocab, _rows.row_stride(logits), _rows.row_stride(out), ignore_index,
             temperature, nat.dtype_code(logits.dtype), int(targets.dtype == torch.int64), nat.dtype_code(out_dtype),
         )
     )

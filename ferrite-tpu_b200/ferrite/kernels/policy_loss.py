@@ -49,13 +49,13 @@ def _launch(logits, targets, rest, clip, coefs, temperature, ignore_index, grad_
     f = torch.empty(4 * rows + 1, dtype=torch.float32, device=dev)  # loss, logp, entropy, kl and the terms of the sum
     base = f.data_ptr()
     clipped = torch.empty(rows, dtype=torch.bool, device=dev)
-    grad = None if grad_dtype is None else torch.empty((rows, vocab), dtype=grad_dtype, device=dev)
+    grad = None if grad_dtype is None else _rows.empty_grad(logits, grad_dtype)
     at = lambda i: base + 4 * (1 + i * rows)  # noqa: E731
     nat.check(
         nat.lib().ferrite_policy_loss(
             nat.stream_ptr(dev), logits.data_ptr(), targets.data_ptr(), old.data_ptr(), adv.data_ptr(), nat.ptr(weights), nat.ptr(ref),
             clip[0], clip[1], coefs[0], coefs[1], temperature, nat.ptr(dloss), grad_scale, base, at(0), at(1), at(2),
-            clipped.data_ptr(), nat.ptr(grad), at(3), 4 * rows, rows, vocab, _rows.row_stride(logits), vocab, ignore_index,
+            clipped.data_ptr(), nat.ptr(grad), at(3), 4 * rows, rows, vocab, _rows.row_stride(logits), vocab if grad is None else _rows.row_stride(grad), ignore_index,
             nat.dtype_code(logits.dtype), int(targets.dtype == torch.int64), -1 if grad_dtype is None else nat.dtype_code(grad_dtype),
         )
     )
