@@ -61,10 +61,10 @@ struct Distill {
 
   // The teacher's softmax over the list, and the student's logits there.
   template <typename TI>
-  __device__ void prep(int64_t r, const Pre& p, const TI* x, const RowIn& in, char* slot) const {
+  __device__ float prep(int64_t r, const Pre& p, const TI* x, const RowIn& in, char* slot) const {
     const List l = list(slot);
     const int lane = threadIdx.x & 31;
-    float m = -INFINITY, bad = 0.f;
+    float m = -INFINITY, bad = 0.f, first = -INFINITY;
     int count = 0;
     for (int j = lane; j < top; j += 32) {
       int64_t i = index(r * ld_list + j);
@@ -75,6 +75,7 @@ struct Distill {
       l.x[j] = i < 0 ? 0.f : DT<TI>::to_f(x[i]);
       l.q[j] = v;
       if (i >= 0) {
+        if (count == 0) first = l.x[j];
         ++count;
         m = fmaxf(m, v);  // a NaN value shows through the sums
       }
@@ -84,6 +85,7 @@ struct Distill {
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
       count += __shfl_xor_sync(0xffffffffu, count, off);
       bad += __shfl_xor_sync(0xffffffffu, bad, off);
+      first = fmaxf(first, __shfl_xor_sync(0xffffffffu, first, off));
     }
     float sum = 0.f, dot = 0.f;
     for (int j = lane; j < top; j += 32) {
@@ -100,6 +102,7 @@ struct Distill {
     }
     for (int j = lane; j < top; j += 32) l.q[j] /= sum;
     if (lane == 0) *reinterpret_cast<Row*>(slot) = Row{p.w, dot / sum - log2f(sum), bad, bad != bad ? max(count, 1) : count};
+    return base_of(first, in);
   }
   __device__ Coef finish(int64_t r, const Norm& w, const RowIn& in, float g, bool writer, char* slot) const {
     const List l = list(slot);
@@ -123,7 +126,7 @@ struct Distill {
     const float f = row.w * tau * g + row.bad;
     cf.A = f * scale;
     cf.B = 0.f;
-    cf.at_t = -f;
+    cf.at_t = -f;  // times a token's weight, added where it is listed
     cf.t = -1;
     cf.masked = row.entries == 0;
     return cf;

@@ -40,8 +40,10 @@ struct LogprobsFwd {
     if (stats) stats[r] = make_float2(0.f, 1.f);
   }
   template <typename TI>
-  __device__ void prep(int64_t, const Pre& p, const TI* x, const RowIn& in, char* slot) const {
-    if ((threadIdx.x & 31) == 0) reinterpret_cast<Row*>(slot)->xt = logit_at(x, p.t, in.vocab);
+  __device__ float prep(int64_t, const Pre& p, const TI* x, const RowIn& in, char* slot) const {
+    const float xt = logit_at(x, p.t, in.vocab);
+    if ((threadIdx.x & 31) == 0) reinterpret_cast<Row*>(slot)->xt = xt;
+    return base_of(xt, in);
   }
   __device__ Coef finish(int64_t r, const Norm& w, const RowIn& in, float, bool writer, char* slot) const {
     if (writer && (threadIdx.x & 31) == 0) {
@@ -66,7 +68,7 @@ struct LogprobsBwd {
   };
   struct Row {
     Norm w;
-    float a, b;
+    float a, b, xt;
     int64_t t;
   };
   __host__ __device__ int slot_bytes() const { return sizeof(Row); }
@@ -74,8 +76,8 @@ struct LogprobsBwd {
   __device__ bool live(const Pre& p) const { return p.t != t.ignore; }
   __device__ void dead(int64_t) const {}
   template <typename TI>
-  __device__ void prep(int64_t r, const Pre& p, const TI*, const RowIn& in, char* slot) const {
-    if ((threadIdx.x & 31) != 0) return;
+  __device__ float prep(int64_t r, const Pre& p, const TI* x, const RowIn& in, char* slot) const {
+    if ((threadIdx.x & 31) != 0) return 0.f;
     Row& w = *reinterpret_cast<Row*>(slot);
     const float2 v = stats[r];
     w.w = Norm{v.x, fabsf(v.y), 0.f, !(v.y > 0.f)};
@@ -86,11 +88,13 @@ struct LogprobsBwd {
       w.b = dentropy[r];
     }
     w.t = p.t;
+    w.xt = logit_at(x, p.t, in.vocab);
+    return 0.f;
   }
   __device__ Norm state(const char* slot) const { return reinterpret_cast<const Row*>(slot)->w; }
   __device__ Coef finish(int64_t, const Norm& w, const RowIn& in, float g, bool, char* slot) const {
     const Row& row = *reinterpret_cast<const Row*>(slot);
-    return coef_of(row.a, row.b, g, row.t, w, in);
+    return coef_of<ENT>(row.a, row.b, g, row.t, row.xt, w, in);
   }
 };
 
@@ -125,9 +129,10 @@ struct Policy {
     clipped[r] = 0;
   }
   template <typename TI>
-  __device__ void prep(int64_t r, const Pre& p, const TI* x, const RowIn& in, char* slot) const {
-    if ((threadIdx.x & 31) == 0)
-      *reinterpret_cast<Row*>(slot) = Row{p.t, p.w, logit_at(x, p.t, in.vocab), old_logp[r], adv[r], ref ? ref[r] : 0.f};
+  __device__ float prep(int64_t r, const Pre& p, const TI* x, const RowIn& in, char* slot) const {
+    const float xt = logit_at(x, p.t, in.vocab);
+    if ((threadIdx.x & 31) == 0) *reinterpret_cast<Row*>(slot) = Row{p.t, p.w, xt, old_logp[r], adv[r], ref ? ref[r] : 0.f};
+    return base_of(xt, in);
   }
   __device__ Coef finish(int64_t r, const Norm& w, const RowIn& in, float g, bool writer, char* slot) const {
     const Row row = *reinterpret_cast<const Row*>(slot);
@@ -150,7 +155,7 @@ struct Policy {
       kl[r] = klv;
       clipped[r] = cut;
     }
-    return coef_of(row.w * da, ENT ? -row.w * ent_coef : 0.f, g, row.t, w, in);
+    return coef_of<ENT>(row.w * da, ENT ? -row.w * ent_coef : 0.f, g, row.t, row.xt, w, in);
   }
 };
 

@@ -8,7 +8,7 @@
 //   kList       the gradient has more single entries than the target's
 //   Pre, pre(r), live(pre), dead(r)   masked rows: not read, results and gradient zero
 //   slot_bytes()                      shared memory of one row
-//   prep(r, pre, x, in, slot)         one warp: what does not need the row's state
+//   prep(r, pre, x, in, slot)         one warp: what does not need the row's state; returns its base
 //   finish(r, norm, in, g, writer, slot)  one warp: the results, written by `writer`; returns the
 //                                       gradient's coefficients in every lane
 //   state(slot)                       kHasStats: the state that prep loaded
@@ -22,8 +22,8 @@
 namespace ferrite {
 namespace rowloss {
 
-// A row cut into 16-byte vectors: `head` elements up to the first 16-byte boundary, nv
-// vectors, and the rest.
+// A row of n elements cut into 16-byte vectors: `head` elements up to the first 16-byte boundary, nv
+// vectors, and the rest.  It goes by the row's address modulo 16 alone.
 template <typename T>
 struct RowCut {
   static constexpr int N = 16 / sizeof(T);
@@ -73,20 +73,25 @@ __global__ void __launch_bounds__(512) row_kernel(RowIn in, RowOut out, Op op) {
       for (int i = tid; i < n; i += nt) dx[i] = DT<TO>::from_f(0.f);
     return;
   }
+  __shared__ float sh_base;
   const RowCut<TI> cut(x, n);
-  if (warp == 0) op.prep(r, pre, x, in, slot);
-  State st = empty_state();
+  if (warp == 0) {
+    const float base = op.prep(r, pre, x, in, slot);
+    if (lane == 0) sh_base = base;
+  }
+  __syncthreads();
+  State st = empty_state(sh_base);
   if constexpr (!Op::kHasStats) {
+    float nc = minus_c(st.m, in);
     for (int v = tid; v < cut.nv; v += nt) {
       float vals[N];
       unpack16<TI>(ld_stream_v4(x + cut.head + v * N), vals);
-      if (v == tid) st.m = vals[0];
-      push<Op::kEnt>(st, vals, in);
+      push<Op::kEnt>(st, nc, vals, in);
     }
     const int e = tid < cut.head ? tid : tid - cut.head + cut.tail;  // an element before or after the vectors
     if (e < cut.head || (tid >= cut.head && e < n)) {
       const float one[1] = {DT<TI>::to_f(x[e])};
-      push<Op::kEnt>(st, one, in);
+      push<Op::kEnt>(st, nc, one, in);
     }
     st = warp_merge<Op::kEnt>(st, in);
     if (lane == 0) sh_state[warp] = st;
@@ -96,7 +101,7 @@ __global__ void __launch_bounds__(512) row_kernel(RowIn in, RowOut out, Op op) {
     __syncwarp();
     Norm w;
     if constexpr (Op::kHasStats) w = op.state(slot);
-    else w = normalise<Op::kEnt>(warp_merge<Op::kEnt>(lane < (nt >> 5) ? sh_state[lane] : empty_state(), in), in);
+    else w = normalise<Op::kEnt>(warp_merge<Op::kEnt>(lane < (nt >> 5) ? sh_state[lane] : empty_state(sh_state[0].m), in), in);
     const float g = GRAD ? (out.dloss ? *out.dloss : 1.f) * out.scale : 0.f;
     const Coef cf = op.finish(r, w, in, g, true, slot);
     if (lane == 0) sh_coef = cf;
@@ -113,12 +118,14 @@ __global__ void __launch_bounds__(512) row_kernel(RowIn in, RowOut out, Op op) {
       const int i = cut.head + v * N;
       float vals[N], d[N];
       unpack16<TI>(ld_stream_v4(x + i), vals);
-      grads_of<Op::kGradEnt>(vals, d, i, in.k, cf);
+      if (cf.big) grads_of<Op::kGradEnt, true>(vals, d, in.k, cf);
+      else grads_of<Op::kGradEnt, false>(vals, d, in.k, cf);
       store_at(dx + i, d, vec);
+      if ((unsigned)(cf.t - i) < (unsigned)N) dx[cf.t] = DT<TO>::from_f(cf.at_t);
     }
     const int e = tid < cut.head ? tid : tid - cut.head + cut.tail;
     if (e < cut.head || (tid >= cut.head && e < n))
-      dx[e] = DT<TO>::from_f(grad_of<Op::kGradEnt>(DT<TI>::to_f(x[e]), in.k, cf) + (e == cf.t ? cf.at_t : 0.f));
+      dx[e] = DT<TO>::from_f(e == cf.t ? cf.at_t : grad_of<Op::kGradEnt>(DT<TI>::to_f(x[e]), in.k, cf));
     if constexpr (Op::kList) {
       __syncthreads();  // the entries below overwrite what another thread has stored
       op.template fix<TO>(cf, dx, 0, n, in, slot, tid, nt);
@@ -135,10 +142,14 @@ __global__ void __launch_bounds__(512) row_kernel(RowIn in, RowOut out, Op op) {
 //
 // A persistent cluster of C CTAs, one CTA to an SM, takes rows cluster, cluster + clusters, ...; each
 // CTA holds 1/C of a row.  C is 1 unless two such slices do not fit a CTA's shared memory.  In a CTA
-//   - one warp issues untiled bulk copies of 16 KB chunks into a ring (mbarriers full / empty), as far
-//     ahead as the ring allows;
-//   - kWarps warps run the passes: the sums of row i chunk by chunk as they land, then the gradient
-//     of row i - 1 from its resident chunks, released one by one.  One row's lag hides everything
+//   - kGroups warps, one for each group below, issue untiled bulk copies of 8 KB chunks into a ring
+//     (mbarriers full / empty), as far ahead as the ring allows.  The ring is a multiple of kGroups
+//     chunks, so that each of its places has one copy warp and one group for good.  (One warp for all of them takes about
+//     600 cycles a chunk -- its waits and its issue, one after the other -- and held reads to 3.7 TB/s.)
+//   - kGroups groups of four warps (one to each of the SM's quarters) run the passes, each on chunks
+//     of its own in turn, so that the warps of a quarter are at different places and keep its fma,
+//     integer and ex2 units busy at once: the sums of row i as its chunks land, then the gradient of
+//     row i - 1 from its resident chunks, released one by one.  One row's lag hides everything
 //     between a row's two passes;
 //   - that is the work of kHelpers warps, row i to helper i mod kHelpers: fetch what the row's loss
 //     needs besides the logits (ahead of time), merge the passes' states (and the C CTAs', through
@@ -148,26 +159,30 @@ __global__ void __launch_bounds__(512) row_kernel(RowIn in, RowOut out, Op op) {
 // no copy is issued, nobody waits, and the copies in flight are waited for before the CTA exits.
 // --------------------------------------------------------------------------
 
-constexpr int kWarps = 16;
-constexpr int kPass = kWarps * 32;              // threads of the passes
-constexpr int kHelpers = 6;
-constexpr int kRingThreads = kPass + 32 + kHelpers * 32;
-constexpr int kChunk = 16384;                   // bytes
+constexpr int kGroups = 4;
+constexpr int kGroup = 128;                     // threads of a group
+constexpr int kPass = kGroups * kGroup;         // threads of the passes
+constexpr int kWarps = kPass / 32;
+constexpr int kHelpers = 4;
+constexpr int kRingThreads = kPass + kGroups * 32 + kHelpers * 32;
+constexpr int kChunk = 8192;                    // bytes
 constexpr int kChunkVec = kChunk / 16;
-constexpr int kVecPer = kChunkVec / kPass;      // vectors a thread takes of a chunk
-constexpr int kMaxChunks = 14;
+constexpr int kVecPer = kChunkVec / kGroup;     // vectors a thread takes of a chunk
+constexpr int kMaxChunks = 28;
+static_assert(kMaxChunks % kGroups == 0 && kMaxChunks <= 32, "places of one group each; a bit for each place");
 constexpr int kRingCluster = 8;
 
 struct RingShared {
   uint64_t full[kMaxChunks], empty[kMaxChunks];
-  // of a helper's row: the passes' states are there; its coefficients are; its gradient is written;
-  // the other CTAs' states are there
+  // of a helper's row: its base is there; the passes' states are; its coefficients are; its
+  // gradient is written; the other CTAs' states are there
   // (two places in turn: a CTA that is a whole turn of the helpers ahead must not reach into a
   // place that another still reads)
-  uint64_t states[kHelpers], done[kHelpers], written[kHelpers], peers[kHelpers][2];
+  uint64_t ready[kHelpers], states[kHelpers], done[kHelpers], written[kHelpers], peers[kHelpers][2];
   State warp_state[kHelpers][kWarps];
   State peer_state[kHelpers][2][kRingCluster];
   Coef coef[kHelpers];
+  float base[kHelpers];
   int abort;
 };
 constexpr int kRingHeader = (int)((sizeof(RingShared) + 127) / 128 * 128);
@@ -187,6 +202,7 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t pa
 // that it takes no issue slots from them.  CLUSTER: other CTAs of the cluster arrive on the barrier.
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait_idle(uint64_t* bar, uint32_t parity, volatile int* abort, int where) {
+  if (CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   while (!(CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity))) {
     if (*abort) return false;
@@ -204,28 +220,34 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
 }
 
 // A row as one CTA of the cluster sees it: its slice of the vectors, and (first and last CTA) the
-// elements before and after them.
+// elements before and after them.  Kept from row to row while the rows' addresses agree modulo 16.
 template <typename T>
 struct Slice {
-  RowCut<T> cut;
-  int v0, nv, chunks;
-  bool first, last;
-  __device__ __forceinline__ Slice(const T* x, int n, int rank, int lg_cluster) : cut(x, n) {
-    const int size = 1 << lg_cluster, per = (cut.nv + size - 1) >> lg_cluster;
-    v0 = min(rank * per, cut.nv);
+  int n, rank, lg, phase;
+  int head, tail, col0, nv, chunks;
+  __device__ __forceinline__ Slice(int n_, int rank_, int lg_) : n(n_), rank(rank_), lg(lg_), phase(-1) {}
+  __device__ __forceinline__ void at(const T* x) {
+    const int p = (int)(reinterpret_cast<uintptr_t>(x) & 15);
+    if (p == phase) return;
+    phase = p;
+    const RowCut<T> cut(x, n);
+    const int per = (cut.nv + (1 << lg) - 1) >> lg, v0 = min(rank * per, cut.nv);
+    head = cut.head;
+    tail = cut.tail;
     nv = min(per, cut.nv - v0);
+    col0 = cut.head + v0 * RowCut<T>::N;
     chunks = (nv + kChunkVec - 1) / kChunkVec;
-    first = rank == 0;
-    last = rank == size - 1;
   }
-  __device__ __forceinline__ int col0() const { return cut.head + v0 * RowCut<T>::N; }
-  __device__ __forceinline__ int lo() const { return first ? 0 : col0(); }
-  __device__ __forceinline__ int hi() const { return last ? cut.n : col0() + nv * RowCut<T>::N; }
+  __device__ __forceinline__ bool first() const { return rank == 0; }
+  __device__ __forceinline__ bool last() const { return rank == (1 << lg) - 1; }
+  __device__ __forceinline__ int lo() const { return first() ? 0 : col0; }
+  __device__ __forceinline__ int hi() const { return last() ? n : col0 + nv * RowCut<T>::N; }
   // the column of the element outside the vectors that thread tid takes, or -1
   __device__ __forceinline__ int edge(int tid) const {
-    if (first && tid < cut.head) return tid;
-    const int e = cut.tail + tid - 16;
-    return last && tid >= 16 && e < cut.n ? e : -1;
+    if (tid >= 32 || (head == 0 && tail == n)) return -1;
+    if (first() && tid < head) return tid;
+    const int e = tail + tid - 16;
+    return last() && tid >= 16 && e < n ? e : -1;
   }
 };
 
@@ -254,9 +276,10 @@ struct LiveRows {
 struct Place {
   int at = 0;
   uint32_t parity = 0;
-  __device__ __forceinline__ void next(int size) {
-    if (++at == size) {
-      at = 0;
+  __device__ __forceinline__ void next(int size, int n = 1) {  // n <= size
+    at += n;
+    if (at >= size) {
+      at -= size;
       parity ^= 1;
     }
   }
@@ -282,9 +305,10 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
   if (tid == 0) {
     for (int i = 0; i < ring_chunks; ++i) {
       mbar_init(&sh.full[i], 1);
-      mbar_init(&sh.empty[i], kWarps);
+      mbar_init(&sh.empty[i], kGroup / 32);
     }
     for (int i = 0; i < kHelpers; ++i) {
+      mbar_init(&sh.ready[i], 1);
       mbar_init(&sh.states[i], kWarps);
       mbar_init(&sh.done[i], 1);
       mbar_init(&sh.written[i], kWarps);
@@ -300,37 +324,49 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
   pdl_wait();
 
   LiveRows<Op> rows{op, in.rows, step};
-  if (warp == kWarps) {  // ---- copies
+  Slice<TI> sl(n, rank, lg_cluster);
+  // registers go where the passes need them: 512 x 96 + 128 x 40 + 128 x 56 = 768 x 80 of the launch
+  if (warp >= kWarps && warp < kWarps + kGroups) {  // ---- copies of one group's chunks
+    setmaxnreg_dec<40>();
+    const int group = warp - kWarps;
     Place p;
-    uint32_t issued = 0;
+    int k = 0;  // which group has the row's first chunk
+    uint32_t used = 0, last_parity = 0;  // bit c: place c has held a copy, and the last one's parity
     bool stop = false;
     for (int64_t r = r0; r < in.rows; r += step) {
-      if (!rows.next(r) || lane != 0 || stop) continue;
+      if (!rows.next(r)) continue;
       const TI* x = static_cast<const TI*>(in.logits) + r * in.ld;
-      const Slice<TI> sl(x, n, rank, lg_cluster);
-      const char* src = reinterpret_cast<const char*>(x + sl.col0());
-      int left = sl.nv;
-      for (int c = 0; c < sl.chunks; ++c) {
-        if (issued >= (uint32_t)ring_chunks && !wait_idle(&sh.empty[p.at], p.parity ^ 1, abort, 201)) {
+      sl.at(x);
+      const int c0 = (group - k + kGroups) % kGroups;
+      Place at = p;
+      at.next(ring_chunks, c0);
+      p.next(ring_chunks, sl.chunks);
+      k = (k + sl.chunks) % kGroups;
+      if (lane != 0 || stop) continue;
+      const char* src = reinterpret_cast<const char*>(x + sl.col0) + c0 * kChunk;
+      int left = sl.nv - c0 * kChunkVec;
+      for (int c = c0; c < sl.chunks; c += kGroups) {
+        // a chunk's first use waits for the barrier's phase before the first: no wait
+        if (!wait_idle(&sh.empty[at.at], at.parity ^ 1, abort, 201)) {
           stop = true;
           break;
         }
         const uint32_t bytes = (uint32_t)min(left, kChunkVec) * 16u;
-        mbar_arrive_expect_tx(&sh.full[p.at], bytes);
-        bulk_load(ring + (size_t)p.at * kChunk, src, bytes, &sh.full[p.at]);
-        src += bytes;
-        left -= kChunkVec;
-        p.next(ring_chunks);
-        ++issued;
+        mbar_arrive_expect_tx(&sh.full[at.at], bytes);
+        bulk_load(ring + (size_t)at.at * kChunk, src, bytes, &sh.full[at.at]);
+        used |= 1u << at.at;
+        last_parity = (last_parity & ~(1u << at.at)) | (at.parity << at.at);
+        at.next(ring_chunks, kGroups);
+        src += kGroups * kChunk;
+        left -= kGroups * kChunkVec;
       }
     }
+    // the last copy into each chunk has landed before the CTA gives up its shared memory
     if (lane == 0) {
-      // the last copy into each chunk has landed before the CTA gives up its shared memory
-      for (int j = 0; j < ring_chunks && (uint32_t)j < issued; ++j) {
-        if (p.at == 0) p.parity ^= 1;
-        p.at = (p.at == 0 ? ring_chunks : p.at) - 1;
+      for (int j = 0; j < ring_chunks; ++j) {
+        if (!(used >> j & 1)) continue;
         const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(&sh.full[p.at], p.parity))
+        while (!mbar_try_wait(&sh.full[j], last_parity >> j & 1))
           if (globaltimer_ns() - t0 > kWaitLimitNs) {
             report_timeout(202);
             *abort = 1;
@@ -338,8 +374,9 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
           }
       }
     }
-  } else if (warp > kWarps) {  // ---- what lies between a row's two passes
-    const int h = warp - kWarps - 1;
+  } else if (warp >= kWarps + kGroups) {  // ---- what lies between a row's two passes
+    setmaxnreg_dec<56>();
+    const int h = warp - kWarps - kGroups;
     char* slot = slots + h * slot_bytes;
     const float g = GRAD ? (out.dloss ? *out.dloss : 1.f) * out.scale : 0.f;
     int turn = 0;
@@ -350,13 +387,17 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
       if (++turn == kHelpers) turn = 0;
       if (!my_turn) continue;
       const TI* x = static_cast<const TI*>(in.logits) + r * in.ld;
-      op.prep(r, op.pre(r), x, in, slot);
+      const float base = op.prep(r, op.pre(r), x, in, slot);
       __syncwarp();
       Norm w;
       if constexpr (kSums) {
+        if (lane == 0) {
+          sh.base[h] = base;
+          mbar_arrive(&sh.ready[h]);
+        }
         (void)wait_idle(&sh.states[h], parity, abort, 203);
         __syncwarp();
-        State st = warp_merge<Op::kEnt>(lane < kWarps ? sh.warp_state[h][lane] : empty_state(), in);
+        State st = warp_merge<Op::kEnt>(lane < kWarps ? sh.warp_state[h][lane] : empty_state(sh.warp_state[h][0].m), in);
         if (cluster > 1) {
           if (lane < cluster) {
             const uint32_t to = mapa_shared(&sh.peer_state[h][half][rank], lane);
@@ -367,7 +408,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
           }
           (void)wait_idle<true>(&sh.peers[h][half], half_parity, abort, 204);
           __syncwarp();
-          st = warp_merge<Op::kEnt>(lane < cluster ? sh.peer_state[h][half][lane] : empty_state(), in);
+          st = warp_merge<Op::kEnt>(lane < cluster ? sh.peer_state[h][half][lane] : empty_state(sh.peer_state[h][half][0].m), in);
           half_parity ^= half;
           half ^= 1;
         }
@@ -389,7 +430,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
         (void)wait_idle(&sh.written[h], parity, abort, 206);
         __syncwarp();
         if (!cf.masked) {
-          const Slice<TI> sl(x, n, rank, lg_cluster);
+          sl.at(x);
           op.template fix<TO>(cf, static_cast<TO*>(out.dlogits) + r * out.ld, sl.lo(), sl.hi(), in, slot, lane, 32);
         }
         __syncwarp();
@@ -397,120 +438,167 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
       parity ^= 1;
     }
   } else {  // ---- the passes
+    setmaxnreg_inc<96>();
+    const int group = warp / (kGroup / 32), gtid = tid % kGroup;
     Place p1, p2, slot1, slot2;  // chunks and helpers of the first and the second pass
+    int k1 = 0, k2 = 0;          // which group has a row's first chunk
     // the second pass of row r: its gradient, from the chunks at p2
     auto second = [&](int64_t r) {
       const TI* x = static_cast<const TI*>(in.logits) + r * in.ld;
+      sl.at(x);
       TO* dx = static_cast<TO*>(out.dlogits) + r * out.ld;
-      const Slice<TI> sl(x, n, rank, lg_cluster);
-      const int col0 = sl.col0(), edge = sl.edge(tid);
-      const bool vec = vector_rows<TO, N>(dx, sl.cut.head);
+      const int col0 = sl.col0, edge = sl.edge(tid);
+      const bool vec = vector_rows<TO, N>(dx, sl.head);
       const float edge_x = edge >= 0 ? DT<TI>::to_f(x[edge]) : 0.f;
       (void)mbar_wait(&sh.done[slot2.at], slot2.parity, abort, 207);
       const Coef cf = sh.coef[slot2.at];
-      int left = sl.nv - tid;
-      TO* to = dx + col0 + tid * N;
-      for (int c = 0; c < sl.chunks; ++c) {
-        if constexpr (!kSums) (void)mbar_wait(&sh.full[p2.at], p2.parity, abort, 208);
-        const uint4* p = reinterpret_cast<const uint4*>(ring + (size_t)p2.at * kChunk) + tid;
-        uint4 raw[kVecPer];
+      const int k2_row = k2, c0 = (group - k2 + kGroups) % kGroups;  // this group's first chunk of the row
+      Place at = p2;
+      p2.next(ring_chunks, sl.chunks);
+      k2 = (k2 + sl.chunks) % kGroups;
+      at.next(ring_chunks, c0);
+      // What is the same for a whole row is decided here, not vector by vector.
+      auto chunks = [&](auto usual_row) {
+        constexpr bool kUsual = decltype(usual_row)::value;
+        int left = sl.nv - c0 * kChunkVec - gtid;
+        TO* to = dx + col0 + (c0 * kChunkVec + gtid) * N;
+        for (int c = c0; c < sl.chunks; c += kGroups) {
+          if constexpr (!kSums) (void)mbar_wait(&sh.full[at.at], at.parity, abort, 208);
+          const uint4* p = reinterpret_cast<const uint4*>(ring + (size_t)at.at * kChunk) + gtid;
+          uint4 raw[kVecPer];
 #pragma unroll
-        for (int q = 0; q < kVecPer; ++q)
-          if (q * kPass < left) raw[q] = p[q * kPass];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.empty[p2.at]);
-        p2.next(ring_chunks);
+          for (int q = 0; q < kVecPer; ++q)
+            if (q * kGroup < left) raw[q] = p[q * kGroup];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[at.at]);
+          at.next(ring_chunks, kGroups);
 #pragma unroll
-        for (int q = 0; q < kVecPer; ++q)
-          if (q * kPass < left) {
-            float vals[N], d[N] = {};
-            unpack16<TI>(raw[q], vals);
-            if (!cf.masked) grads_of<Op::kGradEnt>(vals, d, (int)(to - dx) + q * kPass * N, in.k, cf);
-            store_at(to + q * kPass * N, d, vec);
-          }
-        left -= kChunkVec;
-        to += kChunkVec * N;
-      }
-      if (edge >= 0)
-        dx[edge] = DT<TO>::from_f(cf.masked ? 0.f : grad_of<Op::kGradEnt>(edge_x, in.k, cf) + (edge == cf.t ? cf.at_t : 0.f));
+          for (int q = 0; q < kVecPer; ++q)
+            if (q * kGroup < left) {
+              float vals[N], d[N];
+              unpack16<TI>(raw[q], vals);
+              if constexpr (kUsual) {
+                grads_of<Op::kGradEnt, false>(vals, d, in.k, cf);
+                store_vec<TO, N>(to + q * kGroup * N, d);
+              } else {
+                if (cf.masked) {
+#pragma unroll
+                  for (int j = 0; j < N; ++j) d[j] = 0.f;
+                } else if (cf.big) {
+                  grads_of<Op::kGradEnt, true>(vals, d, in.k, cf);
+                } else {
+                  grads_of<Op::kGradEnt, false>(vals, d, in.k, cf);
+                }
+                store_at(to + q * kGroup * N, d, vec);
+              }
+            }
+          left -= kGroups * kChunkVec;
+          to += kGroups * kChunkVec * N;
+        }
+      };
+      if (vec && !cf.big && !cf.masked) chunks(std::true_type());
+      else chunks(std::false_type());
+      if (edge >= 0) dx[edge] = DT<TO>::from_f(cf.masked ? 0.f : edge == cf.t ? cf.at_t : grad_of<Op::kGradEnt>(edge_x, in.k, cf));
+      // the target's entry, by the thread that has stored the vector it lies in
+      const int tv = (cf.t - col0) / N;
+      if (cf.t >= col0 && tv < sl.nv && tv % kGroup == gtid && (tv / kChunkVec + k2_row) % kGroups == group) dx[cf.t] = DT<TO>::from_f(cf.at_t);
       if constexpr (kFix || !kSums) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.written[slot2.at]);
       }
       slot2.next(kHelpers);
     };
-    int64_t last = -1;  // kLag: the row whose second pass is due
-    for (int64_t r = r0; r < in.rows; r += step) {
-      if (!rows.next(r)) {
+    // the first pass of row r: its sums
+    auto first = [&](int64_t r) {
+      const TI* x = static_cast<const TI*>(in.logits) + r * in.ld;
+      sl.at(x);
+      const int edge = sl.edge(tid);
+      const float edge_x = edge >= 0 ? DT<TI>::to_f(x[edge]) : 0.f;
+      (void)mbar_wait(&sh.ready[slot1.at], slot1.parity, abort, 211);
+      State st = empty_state(sh.base[slot1.at]);
+      float nc = minus_c(st.m, in);
+      const int c0 = (group - k1 + kGroups) % kGroups;
+      Place at = p1;
+      p1.next(ring_chunks, sl.chunks);
+      k1 = (k1 + sl.chunks) % kGroups;
+      at.next(ring_chunks, c0);
+      int left = sl.nv - c0 * kChunkVec - gtid;
+      for (int c = c0; c < sl.chunks; c += kGroups) {
+        (void)mbar_wait(&sh.full[at.at], at.parity, abort, 209);
+        const uint4* p = reinterpret_cast<const uint4*>(ring + (size_t)at.at * kChunk) + gtid;
+        bool by_one = true;
+        if ((kVecPer - 1) * kGroup < left) {  // all of the thread's vectors at once, one check for them
+          uint4 raw[kVecPer];
+#pragma unroll
+          for (int q = 0; q < kVecPer; ++q) raw[q] = p[q * kGroup];
+          uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
+#pragma unroll
+          for (int q = 0; q < kVecPer; ++q) {
+            float vals[N];
+            unpack16<TI>(raw[q], vals);
+            sum_usual<Op::kEnt>(s2, u2, vals, nc, in);
+          }
+          const float s = f2_lo(s2) + f2_hi(s2), u = Op::kEnt ? f2_lo(u2) + f2_hi(u2) : 0.f;
+          if (usual<Op::kEnt>(s, u)) {
+            st.s += s;
+            if constexpr (Op::kEnt) st.u += u;
+            by_one = false;
+          }
+        }
+        if (by_one) {
+#pragma unroll 1
+          for (int q = 0; q < kVecPer; ++q)
+            if (q * kGroup < left) {
+              float vals[N];
+              unpack16<TI>(p[q * kGroup], vals);
+              push<Op::kEnt>(st, nc, vals, in);
+            }
+        }
+        if constexpr (!kLag) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[at.at]);
+        }
+        at.next(ring_chunks, kGroups);
+        left -= kGroups * kChunkVec;
+      }
+      if (edge >= 0) {
+        const float one[1] = {edge_x};
+        push<Op::kEnt>(st, nc, one, in);
+      }
+      __syncwarp();
+      st = warp_merge<Op::kEnt>(st, in);
+      // without a gradient nothing else holds the passes back until the helper has read the
+      // states of the row before in this place
+      if constexpr (!kLag) (void)mbar_wait(&sh.done[slot1.at], slot1.parity ^ 1, abort, 210);
+      if (lane == 0) {
+        sh.warp_state[slot1.at][warp] = st;
+        mbar_arrive(&sh.states[slot1.at]);
+      }
+      slot1.next(kHelpers);
+    };
+    // (one place for each pass, for the instruction cache)
+    int64_t last = -1;  // the row whose second pass is due
+    for (int64_t r = r0;; r += step) {
+      for (; r < in.rows && !rows.next(r); r += step) {  // masked
         if (tid == 0 && rank == 0) op.dead(r);
         if constexpr (GRAD) {
           TO* dx = static_cast<TO*>(out.dlogits) + r * out.ld;
-          const Slice<TI> sl(static_cast<const TI*>(in.logits) + r * in.ld, n, rank, lg_cluster);
-          const bool vec = vector_rows<TO, N>(dx, sl.cut.head);
+          sl.at(static_cast<const TI*>(in.logits) + r * in.ld);
+          const bool vec = vector_rows<TO, N>(dx, sl.head);
           const float zero[N] = {};
-          for (int v = tid; v < sl.nv; v += kPass) store_at(dx + sl.col0() + v * N, zero, vec);
+          for (int v = tid; v < sl.nv; v += kPass) store_at(dx + sl.col0 + v * N, zero, vec);
           const int edge = sl.edge(tid);
           if (edge >= 0) dx[edge] = DT<TO>::from_f(0.f);
         }
-        continue;
       }
-      if constexpr (kSums) {
-        const TI* x = static_cast<const TI*>(in.logits) + r * in.ld;
-        const Slice<TI> sl(x, n, rank, lg_cluster);
-        const int edge = sl.edge(tid);
-        const float edge_x = edge >= 0 ? DT<TI>::to_f(x[edge]) : 0.f;
-        State st = empty_state();
-        int left = sl.nv - tid;
-        for (int c = 0; c < sl.chunks; ++c) {
-          (void)mbar_wait(&sh.full[p1.at], p1.parity, abort, 209);
-          const uint4* p = reinterpret_cast<const uint4*>(ring + (size_t)p1.at * kChunk) + tid;
-          if ((kVecPer - 1) * kPass < left) {
-            float vals[N * kVecPer];
-#pragma unroll
-            for (int q = 0; q < kVecPer; ++q) unpack16<TI>(p[q * kPass], *reinterpret_cast<float(*)[N]>(&vals[q * N]));
-            if (c == 0) st.m = vals[0];
-            push<Op::kEnt>(st, vals, in);
-          } else {
-#pragma unroll
-            for (int q = 0; q < kVecPer - 1; ++q)
-              if (q * kPass < left) {
-                float vals[N];
-                unpack16<TI>(p[q * kPass], vals);
-                if (c == 0 && q == 0) st.m = vals[0];
-                push<Op::kEnt>(st, vals, in);
-              }
-          }
-          if constexpr (!kLag) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.empty[p1.at]);
-          }
-          p1.next(ring_chunks);
-          left -= kChunkVec;
-        }
-        if (edge >= 0) {
-          const float one[1] = {edge_x};
-          push<Op::kEnt>(st, one, in);
-        }
-        __syncwarp();
-        st = warp_merge<Op::kEnt>(st, in);
-        // without a gradient nothing else holds the passes back until the helper has read the
-        // states of the row before in this place
-        if constexpr (!kLag) (void)mbar_wait(&sh.done[slot1.at], slot1.parity ^ 1, abort, 210);
-        if (lane == 0) {
-          sh.warp_state[slot1.at][warp] = st;
-          mbar_arrive(&sh.states[slot1.at]);
-        }
-        slot1.next(kHelpers);
-        if constexpr (kLag) {
-          if (last >= 0) second(last);
-          last = r;
-        }
-      } else {
-        second(r);
-      }
+      const bool more = r < in.rows;
+      if constexpr (!kSums) last = more ? r : -1;
+      else if (more) first(r);
+      if constexpr (GRAD)
+        if (last >= 0) second(last);
+      if (!more) break;
+      if constexpr (kLag) last = r;
     }
-    if constexpr (kLag)
-      if (last >= 0) second(last);
   }
   __syncwarp();
   if (cluster > 1) cluster_sync_all();  // nobody leaves while a peer may still write here
@@ -536,9 +624,10 @@ inline RingPlan plan_ring(int64_t vocab, int elem, int slot_bytes) {
   const int slots = kHelpers * ((slot_bytes + 15) & ~15);
   p.chunks = (kRingSmem - kRingHeader - slots) / kChunk;
   if (p.chunks > kMaxChunks) p.chunks = kMaxChunks;
+  p.chunks -= p.chunks % kGroups;
   p.smem = (size_t)kRingHeader + (size_t)p.chunks * kChunk + slots;
   // two slices are resident, beside lists of up to 1024 entries, and a chunk of the next
-  const int64_t most = (int64_t)(((kRingSmem - kRingHeader - kMaxSlots) / kChunk - 1) / 2) * kChunk;
+  const int64_t most = (int64_t)(((kRingSmem - kRingHeader - kMaxSlots) / kChunk / kGroups * kGroups - kGroups) / 2) * kChunk;
   const int64_t bytes = vocab * elem;
   int lg = 0;
   while ((1 << lg) < kRingCluster && ((bytes + 15) >> lg) + 16 > most) ++lg;

@@ -7,10 +7,12 @@
 //   k = log2(e) / tau,  y_i = k (x_i - m),  e_i = 2^y_i,  s = sum e_i,  u = sum e_i y_i,
 //   logp_i = ln2 (y_i - log2 s),   H = ln2 (log2 s - u / s),   p_i = e_i / s.
 // A row's state is (m, s, u): it is built in one pass and merged pairwise.  m is a base, not the
-// maximum: 2^y keeps its precision over the whole exponent range, so the first element a thread
-// sees serves, and the sums are checked instead -- a sum that reaches 2^80 (an element 2^80 above the
+// maximum: 2^y keeps its precision over the whole exponent range, so any logit of the row's upper
+// part serves, and the sums are checked instead -- a sum that reaches 2^80 (an element 2^80 above the
 // base) is redone against the largest element.  No maximum is taken per element, and no rescaling
-// runs in the usual case.  All of it is f32; only the gradient is rounded, once, on store.
+// runs in the usual case.  The base is the logit of the target (or of the teacher's first token),
+// whose own term is then 1 without rounding.  All of it is f32; only the gradient is rounded, once,
+// on store.
 //
 // y_i is K x_i - c with c = k m rounded -- one number for every term of s and for logp, so that its
 // rounding cancels -- and K = k + k_lo carried to twice f32: the rounding of k alone would shift
@@ -38,7 +40,7 @@ constexpr float kHuge = 0x1p80f;  // a sum above this is redone against the maxi
 struct State {
   float m, s, u;
 };
-__device__ __forceinline__ State empty_state() { return State{-INFINITY, 0.f, 0.f}; }
+__device__ __forceinline__ State empty_state(float base = -INFINITY) { return State{base, 0.f, 0.f}; }
 
 // Rows whose results are asked for.
 struct RowIn {
@@ -64,6 +66,9 @@ struct Targets {
 
 __device__ __forceinline__ bool is_big(float c) { return !(fabsf(c) <= kBig); }
 
+// A logit as a base; -inf (any first element moves it) where it cannot be one.
+__device__ __forceinline__ float base_of(float x, const RowIn& in) { return is_big(x * in.k) ? -INFINITY : x; }
+
 // y of base m1 against base m2 >= m1 (neither -inf): the log2 of the factor that takes sums over
 // to the new base.
 __device__ __forceinline__ float base_step(float m1, float m2, const RowIn& in) {
@@ -88,10 +93,12 @@ __device__ __forceinline__ void rebase(State& st, float m, const RowIn& in) {
 // The states of a warp's lanes merged, in all lanes: one base, one rescaling per lane, plain sums.
 template <bool ENT>
 __device__ __forceinline__ State warp_merge(State st, const RowIn& in) {
-  float m = st.m;
+  if (!__all_sync(0xffffffffu, st.m == __shfl_sync(0xffffffffu, st.m, 0))) {
+    float m = st.m;
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-  rebase<ENT>(st, m, in);
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    rebase<ENT>(st, m, in);
+  }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
     st.s += __shfl_xor_sync(0xffffffffu, st.s, off);
@@ -121,29 +128,46 @@ __device__ __forceinline__ void push_any(State& st, const float (&x)[N], const R
   }
 }
 
-// The same for the usual values: per pair of elements two packed fma (y), two ex2 and packed sums.
+// -k m for the usual values' form of y, or NaN where the base is big (every sum then fails its check).
+__device__ __forceinline__ float minus_c(float m, const RowIn& in) {
+  const float c = m * in.k;
+  return is_big(c) ? __int_as_float(0x7fc00000) : -c;
+}
+
+// Sums of the usual values: per pair of elements two packed fma (y), two ex2 and packed adds.  They
+// count only if usual() holds of them; otherwise the elements go through push_any.
 template <bool ENT, int N>
-__device__ __forceinline__ void push(State& st, const float (&x)[N], const RowIn& in) {
-  if constexpr (N % 2 == 0) {
-    const float c = st.m * in.k;
-    const uint64_t k2 = f2_make(in.k, in.k), l2 = f2_make(in.k_lo, in.k_lo), c2 = f2_make(-c, -c);
-    uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
+__device__ __forceinline__ void sum_usual(uint64_t& s2, uint64_t& u2, const float (&x)[N], float nc, const RowIn& in) {
+  const uint64_t k2 = f2_make(in.k, in.k), l2 = f2_make(in.k_lo, in.k_lo), c2 = f2_make(nc, nc);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const uint64_t x2 = f2_make(x[i], x[i + 1]);
-      const uint64_t y2 = f2_fma(x2, l2, f2_fma(x2, k2, c2));
-      const uint64_t e2 = f2_make(ex2_approx(f2_lo(y2)), ex2_approx(f2_hi(y2)));
-      s2 = f2_add(s2, e2);
-      if constexpr (ENT) u2 = f2_fma(e2, y2, u2);  // -inf: 0 * -inf = NaN, redone below
-    }
+  for (int i = 0; i < N; i += 2) {
+    const uint64_t x2 = f2_make(x[i], x[i + 1]);
+    const uint64_t y2 = f2_fma(x2, l2, f2_fma(x2, k2, c2));
+    const uint64_t e2 = f2_make(ex2_approx(f2_lo(y2)), ex2_approx(f2_hi(y2)));
+    s2 = f2_add(s2, e2);
+    if constexpr (ENT) u2 = f2_fma(e2, y2, u2);  // -inf: 0 * -inf = NaN, and not usual
+  }
+}
+template <bool ENT>
+__device__ __forceinline__ bool usual(float s, float u) {
+  return ENT ? fmaf(fabsf(u), 1.f / 128.f, s) < kHuge : s < kHuge;  // false for NaN
+}
+
+// Adds N elements to a state; nc = minus_c(st.m), kept up to date.
+template <bool ENT, int N>
+__device__ __forceinline__ void push(State& st, float& nc, const float (&x)[N], const RowIn& in) {
+  if constexpr (N % 2 == 0) {
+    uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
+    sum_usual<ENT>(s2, u2, x, nc, in);
     const float s = f2_lo(s2) + f2_hi(s2), u = ENT ? f2_lo(u2) + f2_hi(u2) : 0.f;
-    if (!is_big(c) && s < kHuge && (!ENT || fabsf(u) < kHuge * 128.f)) {
+    if (usual<ENT>(s, u)) {
       st.s += s;
       if constexpr (ENT) st.u += u;
       return;
     }
   }
   push_any<ENT>(st, x, in);
+  nc = minus_c(st.m, in);
 }
 
 // A finished row: base (c, or m where big), s, u.
@@ -208,8 +232,8 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[N]) {
   }
 }
 
-// What the losses of one row hand to its gradient: dx_i = e_i (A + B y_i), and at_t more at i = t,
-// with y_i = k x_i - base, or k (x_i - base) where big.
+// What the losses of one row hand to its gradient: dx_i = e_i (A + B y_i) with y_i = k x_i - base, or
+// k (x_i - base) where big, but at_t at i = t.
 struct Coef {
   float base, A, B;
   float at_t;
@@ -227,10 +251,10 @@ __device__ __forceinline__ float grad_of(float x, float k, const Coef& cf) {
   return e * cf.A;
 }
 
-// Gradients of the N (even) elements x[0, N) at columns i, i + 1, ...
-template <bool ENT, int N>
-__device__ __forceinline__ void grads_of(const float (&x)[N], float (&d)[N], int i, float k, const Coef& cf) {
-  if (cf.big) {
+// Gradients of N (even) elements; BIG as cf.big.
+template <bool ENT, bool BIG, int N>
+__device__ __forceinline__ void grads_of(const float (&x)[N], float (&d)[N], float k, const Coef& cf) {
+  if constexpr (BIG) {
 #pragma unroll
     for (int j = 0; j < N; ++j) d[j] = grad_of<ENT>(x[j], k, cf);
   } else {
@@ -246,11 +270,6 @@ __device__ __forceinline__ void grads_of(const float (&x)[N], float (&d)[N], int
       d[j + 1] = f2_hi(g2);
     }
   }
-  if ((unsigned)(cf.t - i) < (unsigned)N) {
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (i + j == cf.t) d[j] += cf.at_t;
-  }
 }
 
 // The base and common factor of the gradient's y, which leaves k_lo out: k_lo x is taken at the
@@ -264,14 +283,16 @@ __device__ __forceinline__ float grad_base(const Norm& w, const RowIn& in, Coef&
   return ex2_approx((c.base - w.base) + shift);
 }
 // The coefficients for dL/dlogp = a and dL/dH = b: dx = g / tau (a ([i = t] - p_i) - b p_i (log p_i + H)).
-__device__ __forceinline__ Coef coef_of(float a, float b, float g, int64_t t, const Norm& w, const RowIn& in) {
+// ENT: b may differ from 0.  xt: the logit at t.
+template <bool ENT>
+__device__ __forceinline__ Coef coef_of(float a, float b, float g, int64_t t, float xt, const Norm& w, const RowIn& in) {
   const float f = g * in.inv_tau;
   Coef c;
   const float scale = grad_base(w, in, c) / w.s;
   c.t = t >= 0 && t < in.vocab ? (int)t : -1;
-  c.at_t = a * f;
-  c.B = -b * f * kLn2 * scale;
-  c.A = -a * f * scale - c.B * (w.u / w.s);
+  c.B = ENT ? -b * f * kLn2 * scale : 0.f;
+  c.A = -a * f * scale - (ENT ? c.B * (w.u / w.s) : 0.f);
+  c.at_t = grad_of<ENT>(xt, in.k, c) + a * f;
   c.masked = 0;
   return c;
 }

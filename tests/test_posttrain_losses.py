@@ -561,6 +561,53 @@ def test_extreme_ratios_and_margins():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,dtype", [(1500, 32000, "bf16"), (2000, 8200, "bf16"), (900, 8203, "f32"), (700, 50257, "f32"), (600, 131072, "bf16"), (3000, 257, "f16"), (1111, 3001, "bf16")])
+def test_many_rows(rows, vocab, dtype):
+    """More rows than the GPU holds at once, some masked: every row as the plain form has it (f32 sums: the
+    plain form's own error, at most V u, is allowed for besides the kernels'), and no wait of the kernels ran out."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (3 * torch.randn(rows, vocab, device="cuda", generator=g)).to(TORCH[dtype])
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    t[torch.rand(rows, device="cuda", generator=g) < 0.2] = IGN
+    w = torch.rand(rows, device="cuda", generator=g) * (torch.rand(rows, device="cuda", generator=g) > 0.2)
+    old, adv = torch.full((rows,), -9.0, device="cuda"), torch.randn(rows, device="cuda", generator=g)
+    idx = torch.randint(0, vocab, (rows, 40), device="cuda", generator=g)
+    v = torch.randn(rows, 40, device="cuda", generator=g)
+    off = torch.arange(0, rows + 1, rows // 6, device="cuda")[:7]
+    e = 2 * (tol(vocab) + vocab * U) * (1 + np.log(vocab) + 20)
+
+    def near(a, b, scale=1.0):
+        step = rounding(b.float().cpu().numpy().astype(np.float64), dtype) if a.ndim == 2 else 0.0
+        close(a.float(), b.float().cpu().numpy().astype(np.float64), e * scale + 1.01 * step)
+
+    ref = x.detach().float().requires_grad_(True)
+    lp, h = token_logprobs_reference(ref, t)
+    leaf = x.detach().requires_grad_(True)
+    glp, gh = token_logprobs(leaf, t, entropy=True)
+    near(glp.detach(), lp.detach())
+    near(gh.detach(), h.detach())
+    (gr,) = torch.autograd.grad([lp, h], [ref], [adv, 0.1 * adv])
+    (gg,) = torch.autograd.grad([glp, gh], [leaf], [adv, 0.1 * adv])
+    near(gg, gr, 10.0)
+    want = policy_loss_reference(ref, t, old, adv, w, ref_logprobs=old, kl_coef=0.001)
+    (gr,) = torch.autograd.grad(want.loss, ref)
+    got, gg = policy_loss_and_grad(x, t, old, adv, w, ref_logprobs=old, kl_coef=0.001)
+    size = 1 + gr.abs().max().item()
+    near(got.logprobs * (w != 0), want.logprobs)
+    near(gg, gr, 10.0 * size)
+    want = preference_loss_reference(ref, t, old, off)
+    (gr,) = torch.autograd.grad(want.loss, ref)
+    got, gg = preference_loss_and_grad(x, t, old, off)
+    near(gg, gr, 10.0)
+    want = distillation_loss_reference(ref, v, idx, w, temperature=2.0)
+    (gr,) = torch.autograd.grad(want.loss, ref)
+    got, gg = distillation_loss_and_grad(x, v, idx, w, temperature=2.0)
+    near(got.per_token, want.per_token, 10.0)
+    near(gg, gr, 10.0 * size)
+    nat.device_status()
+
+
+@pytest.mark.gpu
 def test_no_rows():
     x = torch.empty(0, 100, device="cuda")
     t, f = torch.empty(0, dtype=torch.long, device="cuda"), torch.empty(0, device="cuda")
