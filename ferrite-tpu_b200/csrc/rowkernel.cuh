@@ -465,22 +465,25 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
         for (int c = c0; c < sl.chunks; c += kGroups) {
           if constexpr (!kSums) (void)mbar_wait(&sh.full[at.at], at.parity, abort, 208);
           const uint4* p = reinterpret_cast<const uint4*>(ring + (size_t)at.at * kChunk) + gtid;
-          uint4 raw[kVecPer];
+          if (kUsual && (kVecPer - 1) * kGroup < left) {  // all of the thread's vectors, side by side
+            uint4 raw[kVecPer];
 #pragma unroll
-          for (int q = 0; q < kVecPer; ++q)
-            if (q * kGroup < left) raw[q] = p[q * kGroup];
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.empty[at.at]);
-          at.next(ring_chunks, kGroups);
+            for (int q = 0; q < kVecPer; ++q) raw[q] = p[q * kGroup];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.empty[at.at]);
 #pragma unroll
-          for (int q = 0; q < kVecPer; ++q)
-            if (q * kGroup < left) {
+            for (int q = 0; q < kVecPer; ++q) {
               float vals[N], d[N];
               unpack16<TI>(raw[q], vals);
-              if constexpr (kUsual) {
-                grads_of<Op::kGradEnt, false>(vals, d, in.k, cf);
-                store_vec<TO, N>(to + q * kGroup * N, d);
-              } else {
+              grads_of<Op::kGradEnt, false>(vals, d, in.k, cf);
+              store_vec<TO, N>(to + q * kGroup * N, d);
+            }
+          } else {
+#pragma unroll 1
+            for (int q = 0; q < kVecPer; ++q)
+              if (q * kGroup < left) {
+                float vals[N], d[N];
+                unpack16<TI>(p[q * kGroup], vals);
                 if (cf.masked) {
 #pragma unroll
                   for (int j = 0; j < N; ++j) d[j] = 0.f;
@@ -491,7 +494,10 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
                 }
                 store_at(to + q * kGroup * N, d, vec);
               }
-            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.empty[at.at]);
+          }
+          at.next(ring_chunks, kGroups);
           left -= kGroups * kChunkVec;
           to += kGroups * kChunkVec * N;
         }
