@@ -140,35 +140,37 @@ __global__ void __launch_bounds__(512) row_kernel(RowIn in, RowOut out, Op op) {
 // gradient) read it there; so traffic is the logits plus the gradient, and the next bound is the
 // ex2 unit (16 a clock and SM: two per element, or one without a gradient).
 //
-// A persistent cluster of C CTAs, one CTA to an SM, takes rows cluster, cluster + clusters, ...; each
-// CTA holds 1/C of a row.  C is 1 unless two such slices do not fit a CTA's shared memory.  In a CTA
+// A persistent cluster of C CTAs, two CTAs to an SM, takes rows cluster, cluster + clusters, ...; each
+// CTA holds 1/C of a row.  C is 1 unless a slice does not fit a CTA's shared memory.  In a CTA
 //   - kGroups warps, one for each group below, issue untiled bulk copies of 8 KB chunks into a ring
 //     (mbarriers full / empty), as far ahead as the ring allows.  The ring is a multiple of kGroups
-//     chunks, so that each of its places has one copy warp and one group for good.  (One warp for all of them takes about
-//     600 cycles a chunk -- its waits and its issue, one after the other -- and held reads to 3.7 TB/s.)
+//     chunks, so that each of its places has one copy warp and one group for good.  (One warp for all
+//     of them takes about 600 cycles a chunk -- its waits and its issue, one after the other -- and
+//     held reads to 3.7 TB/s.)
 //   - kGroups groups of four warps (one to each of the SM's quarters) run the passes, each on chunks
-//     of its own in turn, so that the warps of a quarter are at different places and keep its fma,
-//     integer and ex2 units busy at once: the sums of row i as its chunks land, then the gradient of
-//     row i - 1 from its resident chunks, released one by one.  One row's lag hides everything
-//     between a row's two passes;
-//   - that is the work of kHelpers warps, row i to helper i mod kHelpers: fetch what the row's loss
-//     needs besides the logits (ahead of time), merge the passes' states (and the C CTAs', through
-//     distributed shared memory, in rank order), write the row's results, hand back the gradient's
-//     coefficients, and at last write the single entries of a list.
+//     of its own in turn: the sums of a row as its chunks land, then its gradient from the resident
+//     chunks, released one by one;
+//   - what comes between a row's two passes is the work of kHelpers warps, rows in turn: fetch what
+//     the row's loss needs besides the logits (ahead of time), merge the passes' states (and the C
+//     CTAs', through distributed shared memory, in rank order), write the row's results, hand back
+//     the gradient's coefficients, and at last write the single entries of a list.
+// While one CTA of an SM waits for its helper, the other's passes have the SM.  (One CTA of twice the
+// warps with the gradient a row behind the sums also hides that wait, but pays the fixed part of a
+// row, some 2000 cycles, in twice the warps: 222 us against this form's for 8192 x 32000 bf16.)
 // Every wait is bounded; an expired one raises the CTA's abort flag and the status word, after which
 // no copy is issued, nobody waits, and the copies in flight are waited for before the CTA exits.
 // --------------------------------------------------------------------------
 
-constexpr int kGroups = 4;
+constexpr int kGroups = 2;
 constexpr int kGroup = 128;                     // threads of a group
 constexpr int kPass = kGroups * kGroup;         // threads of the passes
 constexpr int kWarps = kPass / 32;
-constexpr int kHelpers = 4;
+constexpr int kHelpers = 2;
 constexpr int kRingThreads = kPass + kGroups * 32 + kHelpers * 32;
 constexpr int kChunk = 8192;                    // bytes
 constexpr int kChunkVec = kChunk / 16;
 constexpr int kVecPer = kChunkVec / kGroup;     // vectors a thread takes of a chunk
-constexpr int kMaxChunks = 28;
+constexpr int kMaxChunks = 14;
 static_assert(kMaxChunks % kGroups == 0 && kMaxChunks <= 32, "places of one group each; a bit for each place");
 constexpr int kRingCluster = 8;
 
@@ -286,10 +288,10 @@ struct Place {
 };
 
 template <class Op, typename TI, typename TO, bool GRAD>
-__global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut out, Op op, int ring_chunks, int lg_cluster) {
+__global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut out, Op op, int ring_chunks, int lg_cluster) {
   constexpr int N = 16 / sizeof(TI);
   constexpr bool kSums = !Op::kHasStats;        // a first pass
-  constexpr bool kLag = GRAD && kSums;          // both passes: the second one row behind
+  constexpr bool kBoth = GRAD && kSums;         // both passes
   constexpr bool kFix = GRAD && Op::kList;
   extern __shared__ __align__(128) char smem[];
   RingShared& sh = *reinterpret_cast<RingShared*>(smem);
@@ -325,9 +327,10 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
 
   LiveRows<Op> rows{op, in.rows, step};
   Slice<TI> sl(n, rank, lg_cluster);
-  // registers go where the passes need them: 512 x 96 + 128 x 40 + 128 x 56 = 768 x 80 of the launch
-  if (warp >= kWarps && warp < kWarps + kGroups) {  // ---- copies of one group's chunks
-    setmaxnreg_dec<40>();
+  // registers go where the passes need them: 256 x 96 + 128 x 48 = 384 x 80 of the launch
+  if (warp >= kWarps) {
+  setmaxnreg_dec<48>();
+  if (warp < kWarps + kGroups) {  // ---- copies of one group's chunks
     const int group = warp - kWarps;
     Place p;
     int k = 0;  // which group has the row's first chunk
@@ -374,8 +377,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
           }
       }
     }
-  } else if (warp >= kWarps + kGroups) {  // ---- what lies between a row's two passes
-    setmaxnreg_dec<56>();
+  } else {  // ---- what lies between a row's two passes
     const int h = warp - kWarps - kGroups;
     char* slot = slots + h * slot_bytes;
     const float g = GRAD ? (out.dloss ? *out.dloss : 1.f) * out.scale : 0.f;
@@ -437,6 +439,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
       }
       parity ^= 1;
     }
+  }
   } else {  // ---- the passes
     setmaxnreg_inc<96>();
     const int group = warp / (kGroup / 32), gtid = tid % kGroup;
@@ -560,7 +563,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
               push<Op::kEnt>(st, nc, vals, in);
             }
         }
-        if constexpr (!kLag) {
+        if constexpr (!kBoth) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.empty[at.at]);
         }
@@ -575,17 +578,15 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
       st = warp_merge<Op::kEnt>(st, in);
       // without a gradient nothing else holds the passes back until the helper has read the
       // states of the row before in this place
-      if constexpr (!kLag) (void)mbar_wait(&sh.done[slot1.at], slot1.parity ^ 1, abort, 210);
+      if constexpr (!kBoth) (void)mbar_wait(&sh.done[slot1.at], slot1.parity ^ 1, abort, 210);
       if (lane == 0) {
         sh.warp_state[slot1.at][warp] = st;
         mbar_arrive(&sh.states[slot1.at]);
       }
       slot1.next(kHelpers);
     };
-    // (one place for each pass, for the instruction cache)
-    int64_t last = -1;  // the row whose second pass is due
-    for (int64_t r = r0;; r += step) {
-      for (; r < in.rows && !rows.next(r); r += step) {  // masked
+    for (int64_t r = r0; r < in.rows; r += step) {
+      if (!rows.next(r)) {  // masked
         if (tid == 0 && rank == 0) op.dead(r);
         if constexpr (GRAD) {
           TO* dx = static_cast<TO*>(out.dlogits) + r * out.ld;
@@ -596,14 +597,10 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
           const int edge = sl.edge(tid);
           if (edge >= 0) dx[edge] = DT<TO>::from_f(0.f);
         }
+        continue;
       }
-      const bool more = r < in.rows;
-      if constexpr (!kSums) last = more ? r : -1;
-      else if (more) first(r);
-      if constexpr (GRAD)
-        if (last >= 0) second(last);
-      if (!more) break;
-      if constexpr (kLag) last = r;
+      if constexpr (kSums) first(r);
+      if constexpr (GRAD) second(r);
     }
   }
   __syncwarp();
@@ -614,7 +611,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) ring_kernel(RowIn in, RowOut 
 // host
 // --------------------------------------------------------------------------
 
-constexpr int kRingSmem = 227 * 1024;  // all that a CTA can have
+constexpr int kRingSmem = (227 - 2) * 1024 / 2 / 128 * 128;  // of each of two CTAs, besides what the system keeps
 constexpr int kMaxSlots = kHelpers * (64 + 12 * 1024);  // the helpers' lists at their longest
 
 // How rows are split: chunks of each CTA's ring, log2 of the CTAs per row (-1: the row does not fit).
@@ -632,8 +629,8 @@ inline RingPlan plan_ring(int64_t vocab, int elem, int slot_bytes) {
   if (p.chunks > kMaxChunks) p.chunks = kMaxChunks;
   p.chunks -= p.chunks % kGroups;
   p.smem = (size_t)kRingHeader + (size_t)p.chunks * kChunk + slots;
-  // two slices are resident, beside lists of up to 1024 entries, and a chunk of the next
-  const int64_t most = (int64_t)(((kRingSmem - kRingHeader - kMaxSlots) / kChunk / kGroups * kGroups - kGroups) / 2) * kChunk;
+  // a slice is resident, beside lists of up to 1024 entries, and a chunk for each group of the next
+  const int64_t most = (int64_t)((kRingSmem - kRingHeader - kMaxSlots) / kChunk / kGroups * kGroups - kGroups) * kChunk;
   const int64_t bytes = vocab * elem;
   int lg = 0;
   while ((1 << lg) < kRingCluster && ((bytes + 15) >> lg) + 16 > most) ++lg;
