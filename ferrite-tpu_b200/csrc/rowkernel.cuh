@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(512) row_kernel(RowIn in, RowOut out, Op op) {
   }
   __shared__ float sh_base;
   const RowCut<TI> cut(x, n);
+  const Pairs2 kk(in);
   if (warp == 0) {
     const float base = op.prep(r, pre, x, in, slot);
     if (lane == 0) sh_base = base;
@@ -86,12 +87,12 @@ __global__ void __launch_bounds__(512) row_kernel(RowIn in, RowOut out, Op op) {
     for (int v = tid; v < cut.nv; v += nt) {
       float vals[N];
       unpack16<TI>(ld_stream_v4(x + cut.head + v * N), vals);
-      push<Op::kEnt>(st, nc, vals, in);
+      push<Op::kEnt>(st, nc, vals, in, kk);
     }
     const int e = tid < cut.head ? tid : tid - cut.head + cut.tail;  // an element before or after the vectors
     if (e < cut.head || (tid >= cut.head && e < n)) {
       const float one[1] = {DT<TI>::to_f(x[e])};
-      push<Op::kEnt>(st, nc, one, in);
+      push<Op::kEnt>(st, nc, one, in, kk);
     }
     st = warp_merge<Op::kEnt>(st, in);
     if (lane == 0) sh_state[warp] = st;
@@ -118,8 +119,8 @@ __global__ void __launch_bounds__(512) row_kernel(RowIn in, RowOut out, Op op) {
       const int i = cut.head + v * N;
       float vals[N], d[N];
       unpack16<TI>(ld_stream_v4(x + i), vals);
-      if (cf.big) grads_of<Op::kGradEnt, true>(vals, d, in.k, cf);
-      else grads_of<Op::kGradEnt, false>(vals, d, in.k, cf);
+      if (cf.big) grads_of<Op::kGradEnt, true>(vals, d, in.k, cf, kk);
+      else grads_of<Op::kGradEnt, false>(vals, d, in.k, cf, kk);
       store_at(dx + i, d, vec);
       if ((unsigned)(cf.t - i) < (unsigned)N) dx[cf.t] = DT<TO>::from_f(cf.at_t);
     }
@@ -134,6 +135,90 @@ __global__ void __launch_bounds__(512) row_kernel(RowIn in, RowOut out, Op op) {
 }
 
 // --------------------------------------------------------------------------
+// Short rows: a warp per row, which reads it twice (the second time from L1).  No barriers; many rows
+// in flight hide the latency of each.
+// --------------------------------------------------------------------------
+
+constexpr int kShortWarps = 4;                 // rows of a CTA
+constexpr int kShortSlots = 48 * 1024;         // shared memory that their ops may take
+constexpr int kShortRow = 8192;                // bytes: longer rows go to the kernels for whole CTAs
+
+template <class Op, typename TI, typename TO, bool GRAD>
+__global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, RowOut out, Op op) {
+  extern __shared__ __align__(16) char slots[];
+  constexpr int N = 16 / sizeof(TI);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = (int)in.vocab;
+  char* slot = slots + warp * ((op.slot_bytes() + 15) & ~15);
+  const Pairs2 kk(in);
+  const float g = GRAD ? (out.dloss ? *out.dloss : 1.f) * out.scale : 0.f;
+  for (int64_t r = (int64_t)blockIdx.x * kShortWarps + warp; r < in.rows; r += (int64_t)gridDim.x * kShortWarps) {
+    const TI* x = static_cast<const TI*>(in.logits) + r * in.ld;
+    TO* dx = GRAD ? static_cast<TO*>(out.dlogits) + r * out.ld : nullptr;
+    const RowCut<TI> cut(x, n);
+    const bool vec = GRAD && vector_rows<TO, N>(dx, cut.head);
+    const int e0 = lane < cut.head ? lane : lane - cut.head + cut.tail;  // an element before or after the vectors
+    const int edge = e0 < cut.head || (lane >= cut.head && e0 < n) ? e0 : -1;
+    auto zeros = [&]() {
+      if constexpr (GRAD) {
+        const float zero[N] = {};
+        for (int v = lane; v < cut.nv; v += 32) store_at(dx + cut.head + v * N, zero, vec);
+        if (edge >= 0) dx[edge] = DT<TO>::from_f(0.f);
+      }
+    };
+    const auto pre = op.pre(r);
+    if (!op.live(pre)) {
+      if (lane == 0) op.dead(r);
+      zeros();
+      continue;
+    }
+    __syncwarp();  // the slot is still being read for the row before
+    State st = empty_state(op.prep(r, pre, x, in, slot));
+    __syncwarp();
+    const float edge_x = edge >= 0 ? DT<TI>::to_f(x[edge]) : 0.f;
+    Norm w;
+    if constexpr (Op::kHasStats) {
+      w = op.state(slot);
+    } else {
+      float nc = minus_c(st.m, in);
+      for (int v = lane; v < cut.nv; v += 32) {
+        float vals[N];
+        unpack16<TI>(ld_v4(x + cut.head + v * N), vals);
+        push<Op::kEnt>(st, nc, vals, in, kk);
+      }
+      if (edge >= 0) {
+        const float one[1] = {edge_x};
+        push<Op::kEnt>(st, nc, one, in, kk);
+      }
+      __syncwarp();
+      w = normalise<Op::kEnt>(warp_merge<Op::kEnt>(st, in), in);
+    }
+    const Coef cf = op.finish(r, w, in, g, true, slot);
+    if constexpr (GRAD) {
+      if (cf.masked) {
+        zeros();
+        continue;
+      }
+      for (int v = lane; v < cut.nv; v += 32) {
+        const int i = cut.head + v * N;
+        float vals[N], d[N];
+        unpack16<TI>(ld_v4(x + i), vals);
+        if (cf.big) grads_of<Op::kGradEnt, true>(vals, d, in.k, cf, kk);
+        else grads_of<Op::kGradEnt, false>(vals, d, in.k, cf, kk);
+        store_at(dx + i, d, vec);
+        if ((unsigned)(cf.t - i) < (unsigned)N) dx[cf.t] = DT<TO>::from_f(cf.at_t);
+      }
+      if (edge >= 0) dx[edge] = DT<TO>::from_f(edge == cf.t ? cf.at_t : grad_of<Op::kGradEnt>(edge_x, in.k, cf));
+      if constexpr (Op::kList) {
+        __syncwarp();  // the entries below overwrite what another lane has stored
+        op.template fix<TO>(cf, dx, 0, n, in, slot, lane, 32);
+      }
+    }
+  }
+}
+
+// --------------------------------------------------------------------------
 // Rows that fit: one read, one write.
 //
 // Bound: HBM.  A row is read once into shared memory, and both passes (the sums, then the
@@ -142,11 +227,11 @@ __global__ void __launch_bounds__(512) row_kernel(RowIn in, RowOut out, Op op) {
 //
 // A persistent cluster of C CTAs, two CTAs to an SM, takes rows cluster, cluster + clusters, ...; each
 // CTA holds 1/C of a row.  C is 1 unless a slice does not fit a CTA's shared memory.  In a CTA
-//   - kGroups warps, one for each group below, issue untiled bulk copies of 8 KB chunks into a ring
+//   - kGroups warps, one for each group below, issue untiled bulk copies of 16 KB chunks into a ring
 //     (mbarriers full / empty), as far ahead as the ring allows.  The ring is a multiple of kGroups
 //     chunks, so that each of its places has one copy warp and one group for good.  (One warp for all
-//     of them takes about 600 cycles a chunk -- its waits and its issue, one after the other -- and
-//     held reads to 3.7 TB/s.)
+//     of them takes about 600 cycles a copy -- its waits and its issue, one after the other -- and
+//     held reads to 3.7 TB/s with 8 KB copies.)
 //   - kGroups groups of four warps (one to each of the SM's quarters) run the passes, each on chunks
 //     of its own in turn: the sums of a row as its chunks land, then its gradient from the resident
 //     chunks, released one by one;
@@ -167,10 +252,10 @@ constexpr int kPass = kGroups * kGroup;         // threads of the passes
 constexpr int kWarps = kPass / 32;
 constexpr int kHelpers = 2;
 constexpr int kRingThreads = kPass + kGroups * 32 + kHelpers * 32;
-constexpr int kChunk = 8192;                    // bytes
+constexpr int kChunk = 16384;                   // bytes
 constexpr int kChunkVec = kChunk / 16;
 constexpr int kVecPer = kChunkVec / kGroup;     // vectors a thread takes of a chunk
-constexpr int kMaxChunks = 14;
+constexpr int kMaxChunks = 6;
 static_assert(kMaxChunks % kGroups == 0 && kMaxChunks <= 32, "places of one group each; a bit for each place");
 constexpr int kRingCluster = 8;
 
@@ -183,7 +268,7 @@ struct RingShared {
   uint64_t ready[kHelpers], states[kHelpers], done[kHelpers], written[kHelpers], peers[kHelpers][2];
   State warp_state[kHelpers][kWarps];
   State peer_state[kHelpers][2][kRingCluster];
-  Coef coef[kHelpers];
+  alignas(16) Coef coef[kHelpers];
   float base[kHelpers];
   int abort;
 };
@@ -327,9 +412,9 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
 
   LiveRows<Op> rows{op, in.rows, step};
   Slice<TI> sl(n, rank, lg_cluster);
-  // registers go where the passes need them: 256 x 96 + 128 x 48 = 384 x 80 of the launch
+  // registers go where the passes need them: 256 x 88 + 128 x 64 = 384 x 80 of the launch
   if (warp >= kWarps) {
-  setmaxnreg_dec<48>();
+  setmaxnreg_dec<64>();
   if (warp < kWarps + kGroups) {  // ---- copies of one group's chunks
     const int group = warp - kWarps;
     Place p;
@@ -441,7 +526,8 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
     }
   }
   } else {  // ---- the passes
-    setmaxnreg_inc<96>();
+    setmaxnreg_inc<88>();
+    const Pairs2 kk(in);
     const int group = warp / (kGroup / 32), gtid = tid % kGroup;
     Place p1, p2, slot1, slot2;  // chunks and helpers of the first and the second pass
     int k1 = 0, k2 = 0;          // which group has a row's first chunk
@@ -468,7 +554,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
         for (int c = c0; c < sl.chunks; c += kGroups) {
           if constexpr (!kSums) (void)mbar_wait(&sh.full[at.at], at.parity, abort, 208);
           const uint4* p = reinterpret_cast<const uint4*>(ring + (size_t)at.at * kChunk) + gtid;
-          if (kUsual && (kVecPer - 1) * kGroup < left) {  // all of the thread's vectors, side by side
+          if constexpr (kUsual) {  // all of the thread's vectors, side by side
             uint4 raw[kVecPer];
 #pragma unroll
             for (int q = 0; q < kVecPer; ++q) raw[q] = p[q * kGroup];
@@ -478,8 +564,8 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
             for (int q = 0; q < kVecPer; ++q) {
               float vals[N], d[N];
               unpack16<TI>(raw[q], vals);
-              grads_of<Op::kGradEnt, false>(vals, d, in.k, cf);
-              store_vec<TO, N>(to + q * kGroup * N, d);
+              grads_of<Op::kGradEnt, false>(vals, d, in.k, cf, kk);
+              if (q * kGroup < left) store_vec<TO, N>(to + q * kGroup * N, d);
             }
           } else {
 #pragma unroll 1
@@ -491,9 +577,9 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
 #pragma unroll
                   for (int j = 0; j < N; ++j) d[j] = 0.f;
                 } else if (cf.big) {
-                  grads_of<Op::kGradEnt, true>(vals, d, in.k, cf);
+                  grads_of<Op::kGradEnt, true>(vals, d, in.k, cf, kk);
                 } else {
-                  grads_of<Op::kGradEnt, false>(vals, d, in.k, cf);
+                  grads_of<Op::kGradEnt, false>(vals, d, in.k, cf, kk);
                 }
                 store_at(to + q * kGroup * N, d, vec);
               }
@@ -526,6 +612,12 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
       (void)mbar_wait(&sh.ready[slot1.at], slot1.parity, abort, 211);
       State st = empty_state(sh.base[slot1.at]);
       float nc = minus_c(st.m, in);
+      // What stands for the elements past the row's end in its last chunk: nothing of the sums.  -inf,
+      // but in 0 * y where the entropy is summed -1e30; f16 has none that is small enough for every
+      // temperature, and sums such a chunk vector by vector.
+      constexpr bool kPad = !Op::kEnt || !std::is_same_v<TI, __half>;
+      const uint32_t pad = std::is_same_v<TI, float> ? (Op::kEnt ? 0xf149f2cau : 0xff800000u)
+                           : std::is_same_v<TI, __half> ? 0xfc00fc00u : (Op::kEnt ? 0xf149f149u : 0xff80ff80u);
       const int c0 = (group - k1 + kGroups) % kGroups;
       Place at = p1;
       p1.next(ring_chunks, sl.chunks);
@@ -536,16 +628,19 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
         (void)mbar_wait(&sh.full[at.at], at.parity, abort, 209);
         const uint4* p = reinterpret_cast<const uint4*>(ring + (size_t)at.at * kChunk) + gtid;
         bool by_one = true;
-        if ((kVecPer - 1) * kGroup < left) {  // all of the thread's vectors at once, one check for them
+        if (kPad || (kVecPer - 1) * kGroup < left) {  // all of the thread's vectors at once, one check for them
           uint4 raw[kVecPer];
 #pragma unroll
-          for (int q = 0; q < kVecPer; ++q) raw[q] = p[q * kGroup];
+          for (int q = 0; q < kVecPer; ++q) {
+            raw[q] = p[q * kGroup];  // past the row's end: whatever the chunk holds
+            if (kPad && q * kGroup >= left) raw[q] = make_uint4(pad, pad, pad, pad);
+          }
           uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
 #pragma unroll
           for (int q = 0; q < kVecPer; ++q) {
             float vals[N];
             unpack16<TI>(raw[q], vals);
-            sum_usual<Op::kEnt>(s2, u2, vals, nc, in);
+            sum_usual<Op::kEnt>(s2, u2, vals, nc, kk);
           }
           const float s = f2_lo(s2) + f2_hi(s2), u = Op::kEnt ? f2_lo(u2) + f2_hi(u2) : 0.f;
           if (usual<Op::kEnt>(s, u)) {
@@ -560,7 +655,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
             if (q * kGroup < left) {
               float vals[N];
               unpack16<TI>(p[q * kGroup], vals);
-              push<Op::kEnt>(st, nc, vals, in);
+              push<Op::kEnt>(st, nc, vals, in, kk);
             }
         }
         if constexpr (!kBoth) {
@@ -572,7 +667,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
       }
       if (edge >= 0) {
         const float one[1] = {edge_x};
-        push<Op::kEnt>(st, nc, one, in);
+        push<Op::kEnt>(st, nc, one, in, kk);
       }
       __syncwarp();
       st = warp_merge<Op::kEnt>(st, in);
@@ -629,8 +724,8 @@ inline RingPlan plan_ring(int64_t vocab, int elem, int slot_bytes) {
   if (p.chunks > kMaxChunks) p.chunks = kMaxChunks;
   p.chunks -= p.chunks % kGroups;
   p.smem = (size_t)kRingHeader + (size_t)p.chunks * kChunk + slots;
-  // a slice is resident, beside lists of up to 1024 entries, and a chunk for each group of the next
-  const int64_t most = (int64_t)((kRingSmem - kRingHeader - kMaxSlots) / kChunk / kGroups * kGroups - kGroups) * kChunk;
+  // a slice is resident, beside lists of up to 1024 entries (short ones leave two more chunks, for the next row)
+  const int64_t most = (int64_t)((kRingSmem - kRingHeader - kMaxSlots) / kChunk / kGroups * kGroups) * kChunk;
   const int64_t bytes = vocab * elem;
   int lg = 0;
   while ((1 << lg) < kRingCluster && ((bytes + 15) >> lg) + 16 > most) ++lg;
@@ -638,7 +733,7 @@ inline RingPlan plan_ring(int64_t vocab, int elem, int slot_bytes) {
   return p;
 }
 
-inline int row_threads(int64_t vocab) { return vocab <= 1024 ? 64 : vocab <= 4096 ? 128 : vocab <= 16384 ? 256 : 512; }
+inline int row_threads(int64_t vocab) { return vocab <= 4096 ? 128 : vocab <= 16384 ? 256 : 512; }
 
 template <class Op, typename TI, typename TO, bool GRAD>
 static int launch_row(cudaStream_t s, const RowIn& in, const RowOut& out, const Op& op, const char* name) {
@@ -646,7 +741,12 @@ static int launch_row(cudaStream_t s, const RowIn& in, const RowOut& out, const 
   if (dev < 0 || dev >= 64) return fail(FERRITE_LAUNCH_FAILED, "%s: device ordinal %d", name, dev);
   cudaError_t e;
   const RingPlan p = plan_ring(in.vocab, sizeof(TI), op.slot_bytes());
-  if (in.vocab * (int64_t)sizeof(TI) >= 8192 && p.lg_cluster >= 0) {
+  const int64_t bytes = in.vocab * (int64_t)sizeof(TI);
+  const int slots = kShortWarps * ((op.slot_bytes() + 15) & ~15);
+  if (bytes < kShortRow && slots <= kShortSlots) {
+    const int64_t ctas = (in.rows + kShortWarps - 1) / kShortWarps, most = (int64_t)num_sms(dev) * 16;
+    e = launch_pdl(short_row_kernel<Op, TI, TO, GRAD>, dim3((unsigned)(ctas < most ? ctas : most)), dim3(kShortWarps * 32), slots, s, in, out, op);
+  } else if (bytes >= kShortRow && p.lg_cluster >= 0) {
     auto kern = ring_kernel<Op, TI, TO, GRAD>;
     // clusters of each size that are resident at once, per device (set once; racing first calls
     // store the same values): a persistent grid of more would run its last ones after the others

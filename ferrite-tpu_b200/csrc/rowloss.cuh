@@ -134,15 +134,21 @@ __device__ __forceinline__ float minus_c(float m, const RowIn& in) {
   return is_big(c) ? __int_as_float(0x7fc00000) : -c;
 }
 
+// k and k_lo in both halves of register pairs.
+struct Pairs2 {
+  uint64_t k, k_lo;
+  __device__ __forceinline__ explicit Pairs2(const RowIn& in) : k(f2_make(in.k, in.k)), k_lo(f2_make(in.k_lo, in.k_lo)) {}
+};
+
 // Sums of the usual values: per pair of elements two packed fma (y), two ex2 and packed adds.  They
 // count only if usual() holds of them; otherwise the elements go through push_any.
 template <bool ENT, int N>
-__device__ __forceinline__ void sum_usual(uint64_t& s2, uint64_t& u2, const float (&x)[N], float nc, const RowIn& in) {
-  const uint64_t k2 = f2_make(in.k, in.k), l2 = f2_make(in.k_lo, in.k_lo), c2 = f2_make(nc, nc);
+__device__ __forceinline__ void sum_usual(uint64_t& s2, uint64_t& u2, const float (&x)[N], float nc, const Pairs2& kk) {
+  const uint64_t c2 = f2_make(nc, nc);
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
     const uint64_t x2 = f2_make(x[i], x[i + 1]);
-    const uint64_t y2 = f2_fma(x2, l2, f2_fma(x2, k2, c2));
+    const uint64_t y2 = f2_fma(x2, kk.k_lo, f2_fma(x2, kk.k, c2));
     const uint64_t e2 = f2_make(ex2_approx(f2_lo(y2)), ex2_approx(f2_hi(y2)));
     s2 = f2_add(s2, e2);
     if constexpr (ENT) u2 = f2_fma(e2, y2, u2);  // -inf: 0 * -inf = NaN, and not usual
@@ -155,10 +161,10 @@ __device__ __forceinline__ bool usual(float s, float u) {
 
 // Adds N elements to a state; nc = minus_c(st.m), kept up to date.
 template <bool ENT, int N>
-__device__ __forceinline__ void push(State& st, float& nc, const float (&x)[N], const RowIn& in) {
+__device__ __forceinline__ void push(State& st, float& nc, const float (&x)[N], const RowIn& in, const Pairs2& kk) {
   if constexpr (N % 2 == 0) {
     uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
-    sum_usual<ENT>(s2, u2, x, nc, in);
+    sum_usual<ENT>(s2, u2, x, nc, kk);
     const float s = f2_lo(s2) + f2_hi(s2), u = ENT ? f2_lo(u2) + f2_hi(u2) : 0.f;
     if (usual<ENT>(s, u)) {
       st.s += s;
@@ -234,7 +240,7 @@ __device__ __forceinline__ void store_vec(T* p, const float (&f)[N]) {
 
 // What the losses of one row hand to its gradient: dx_i = e_i (A + B y_i) with y_i = k x_i - base, or
 // k (x_i - base) where big, but at_t at i = t.
-struct Coef {
+struct alignas(16) Coef {
   float base, A, B;
   float at_t;
   int t;            // no single entry: negative
@@ -253,15 +259,15 @@ __device__ __forceinline__ float grad_of(float x, float k, const Coef& cf) {
 
 // Gradients of N (even) elements; BIG as cf.big.
 template <bool ENT, bool BIG, int N>
-__device__ __forceinline__ void grads_of(const float (&x)[N], float (&d)[N], float k, const Coef& cf) {
+__device__ __forceinline__ void grads_of(const float (&x)[N], float (&d)[N], float k, const Coef& cf, const Pairs2& kk) {
   if constexpr (BIG) {
 #pragma unroll
     for (int j = 0; j < N; ++j) d[j] = grad_of<ENT>(x[j], k, cf);
   } else {
-    const uint64_t k2 = f2_make(k, k), c2 = f2_make(-cf.base, -cf.base), A2 = f2_make(cf.A, cf.A), B2 = f2_make(cf.B, cf.B);
+    const uint64_t c2 = f2_make(-cf.base, -cf.base), A2 = f2_make(cf.A, cf.A), B2 = f2_make(cf.B, cf.B);
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
-      const uint64_t y2 = f2_fma(f2_make(x[j], x[j + 1]), k2, c2);
+      const uint64_t y2 = f2_fma(f2_make(x[j], x[j + 1]), kk.k, c2);
       const uint64_t e2 = f2_make(ex2_approx(f2_lo(y2)), ex2_approx(f2_hi(y2)));
       uint64_t g2 = A2;
       if constexpr (ENT) g2 = f2_fma(B2, f2_make(fmaxf(f2_lo(y2), -1000.f), fmaxf(f2_hi(y2), -1000.f)), A2);
