@@ -11,6 +11,7 @@ namespace ferrite {
 namespace rowloss {
 
 constexpr int kMaxTop = 1024;
+constexpr int kSeenWords = 256;
 
 struct Distill {
   static constexpr bool kEnt = false, kGradEnt = false, kHasStats = false, kList = true, kForwardOnly = false;
@@ -27,11 +28,13 @@ struct Distill {
     float w;
   };
   // A row in shared memory: this, then q, the student's logits at the listed tokens, the tokens.
-  struct Row {
+  struct alignas(16) Row {
+    uint32_t seen[kSeenWords];  // a bit for each token's hash
     float w;
-    float qlogq;  // sum_j q_j log2 q_j
-    float bad;    // NaN if an index is out of range
-    int entries;  // 0: a masked row
+    float qlogq;   // sum_j q_j log2 q_j
+    float bad;     // NaN if an index is out of range
+    int16_t entries;  // 0: a masked row
+    int16_t twice;    // a token is listed more than once
   };
   struct List {
     float* q;
@@ -45,6 +48,29 @@ struct Distill {
     l.x = l.q + top;
     l.idx = reinterpret_cast<int*>(l.x + top);
     return l;
+  }
+  // Whether a token is listed more than once.  Each entry sets its token's bit in a table of 2^13
+  // hashes; an entry that finds its bit set (a token's second, or a chance hit) is compared with the
+  // whole list.  (Comparing every entry with every other took 9 us a row at 128 entries, more than
+  // the row itself.)
+  __device__ bool any_twice(Row& row, const List& l) const {
+    const int lane = threadIdx.x & 31;
+    for (int j = lane; j < kSeenWords; j += 32) row.seen[j] = 0;
+    __syncwarp();
+    bool twice = false;
+    for (int j0 = 0; j0 < top; j0 += 32) {
+      const int mine = j0 + lane < top ? l.idx[j0 + lane] : -1;
+      bool hit = false;
+      if (mine >= 0) {
+        const uint32_t hash = ((uint32_t)mine * 2654435761u) >> 19, bit = 1u << (hash & 31);
+        hit = atomicOr(&row.seen[hash >> 5], bit) & bit;
+      }
+      for (uint32_t hits = __ballot_sync(0xffffffffu, hit); hits; hits &= hits - 1) {
+        const int at = __ffs(hits) - 1, token = __shfl_sync(0xffffffffu, mine, at);
+        for (int o = lane; o < top; o += 32) twice |= o != j0 + at && l.idx[o] == token;
+      }
+    }
+    return __any_sync(0xffffffffu, twice);
   }
 
   __device__ float value(int64_t i) const {
@@ -101,12 +127,21 @@ struct Distill {
       dot += __shfl_xor_sync(0xffffffffu, dot, off);
     }
     for (int j = lane; j < top; j += 32) l.q[j] /= sum;
-    if (lane == 0) *reinterpret_cast<Row*>(slot) = Row{p.w, dot / sum - log2f(sum), bad, bad != bad ? max(count, 1) : count};
+    Row& row = *reinterpret_cast<Row*>(slot);
+    __syncwarp();
+    const bool twice = any_twice(row, l);
+    if (lane == 0) {
+      row.w = p.w;
+      row.qlogq = dot / sum - log2f(sum);
+      row.bad = bad;
+      row.entries = (int16_t)(bad != bad ? max(count, 1) : count);
+      row.twice = twice;
+    }
     return base_of(first, in);
   }
   __device__ Coef finish(int64_t r, const Norm& w, const RowIn& in, float g, bool writer, char* slot) const {
     const List l = list(slot);
-    const Row row = *reinterpret_cast<const Row*>(slot);
+    const Row& row = *reinterpret_cast<const Row*>(slot);
     Coef cf;
     const float scale = grad_base(w, in, cf) / w.s;
     if (writer) {
@@ -131,17 +166,20 @@ struct Distill {
     cf.masked = row.entries == 0;
     return cf;
   }
-  // The listed tokens' entries in [lo, hi), by threads tid < threads: the thread of entry j sums the
-  // weights of every entry with the same token, so that a token listed twice is written the same
-  // value twice.
+  // The listed tokens' entries in [lo, hi), by threads tid < threads.  Where a token is listed twice, the
+  // thread of each of its entries sums all their weights, and writes the same value.
   template <typename TO>
   __device__ void fix(const Coef& cf, TO* dx, int lo, int hi, const RowIn& in, char* slot, int tid, int threads) const {
     const List l = list(slot);
+    const bool twice = reinterpret_cast<const Row*>(slot)->twice;
     for (int j = tid; j < top; j += threads) {
       const int i = l.idx[j];
       if (i < lo || i >= hi) continue;  // absent entries too: lo is not negative
-      float q = 0.f;
-      for (int o = 0; o < top; ++o) q += l.idx[o] == i ? l.q[o] : 0.f;
+      float q = l.q[j];
+      if (twice) {
+        q = 0.f;
+        for (int o = 0; o < top; ++o) q += l.idx[o] == i ? l.q[o] : 0.f;
+      }
       dx[i] = DT<TO>::from_f(fmaf(cf.at_t, q, grad_of<false>(l.x[j], in.k, cf)));
     }
   }

@@ -270,6 +270,20 @@ __global__ void __launch_bounds__(kPairThreads) pairs_kernel(Pairs a) {
     for (int64_t i = hi[1] + threadIdx.x; i < a.rows; i += blockDim.x) a.coef[i] = 0.f;
 }
 
+static int check_pairs(const char* op, const float* logp, const float* ref_logp, const void* targets, const int64_t* offsets, float beta,
+                       float label_smoothing, int kind, const float* loss, const float* margins, const float* workspace, size_t workspace_bytes,
+                       int64_t rows, int64_t pairs, int target_dtype) {
+  if (rows < 0 || pairs < 1 || pairs > 0x3fffffff) return fail(FERRITE_BAD_SHAPE, "%s: rows=%lld pairs=%lld", op, (long long)rows, (long long)pairs);
+  if (int rc = check_targets(op, target_dtype)) return rc;
+  if (kind < 0 || kind > 2) return fail(FERRITE_BAD_SHAPE, "%s: kind %d (0 sigmoid, 1 squared, 2 hinge)", op, kind);
+  if (!(beta > 0.f) || !std::isfinite(beta)) return fail(FERRITE_BAD_SHAPE, "%s: beta %g (it must be positive)", op, (double)beta);
+  if (!(label_smoothing >= 0.f && label_smoothing < 0.5f)) return fail(FERRITE_BAD_SHAPE, "%s: label_smoothing %g (0 <= it < 0.5)", op, (double)label_smoothing);
+  if (workspace_bytes < (size_t)pairs * sizeof(float)) return fail(FERRITE_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %lld needed", op, workspace_bytes, (long long)pairs * 4);
+  if (!offsets || !loss || !margins || !workspace || (rows > 0 && (!logp || !ref_logp || !targets)))
+    return fail(FERRITE_BAD_SHAPE, "%s: null pointer", op);
+  return FERRITE_OK;
+}
+
 }  // namespace rowloss
 
 FERRITE_DEFINE_STATUS_READER(status_logprobs)
@@ -352,20 +366,37 @@ int ferrite_preference_pairs(void* stream, const float* logp, const float* ref_l
                              float* workspace, size_t workspace_bytes, int64_t rows, int64_t pairs, int64_t ignore_index, int target_dtype) {
   const char* op = "preference_pairs";
   if (int rc = injected_fault(op)) return rc;
-  if (rows < 0 || pairs < 1 || pairs > 0x3fffffff) return fail(FERRITE_BAD_SHAPE, "%s: rows=%lld pairs=%lld", op, (long long)rows, (long long)pairs);
-  if (int rc = check_targets(op, target_dtype)) return rc;
-  if (kind < 0 || kind > 2) return fail(FERRITE_BAD_SHAPE, "%s: kind %d (0 sigmoid, 1 squared, 2 hinge)", op, kind);
-  if (!(beta > 0.f) || !std::isfinite(beta)) return fail(FERRITE_BAD_SHAPE, "%s: beta %g (it must be positive)", op, (double)beta);
-  if (!(label_smoothing >= 0.f && label_smoothing < 0.5f)) return fail(FERRITE_BAD_SHAPE, "%s: label_smoothing %g (0 <= it < 0.5)", op, (double)label_smoothing);
-  if (workspace_bytes < (size_t)pairs * sizeof(float)) return fail(FERRITE_WORKSPACE_TOO_SMALL, "%s: workspace of %zu bytes, %lld needed", op, workspace_bytes, (long long)pairs * 4);
-  if (!offsets || !loss || !margins || !workspace || (rows > 0 && (!logp || !ref_logp || !targets)))
-    return fail(FERRITE_BAD_SHAPE, "%s: null pointer", op);
+  if (int rc = check_pairs(op, logp, ref_logp, targets, offsets, beta, label_smoothing, kind, loss, margins, workspace, workspace_bytes, rows, pairs, target_dtype))
+    return rc;
   cudaStream_t s = (cudaStream_t)stream;
   const Pairs a{logp, ref_logp, Targets{targets, target_dtype, ignore_index}, offsets, workspace, margins, coef, rows, pairs, beta, label_smoothing, kind, average};
   const cudaError_t e = launch_pdl(pairs_kernel, dim3((unsigned)pairs), dim3(kPairThreads), 0, s, a);
   if (e != cudaSuccess) return fail(FERRITE_LAUNCH_FAILED, "%s: %s", op, cudaGetErrorString(e));
   if (int rc = check_launch(op)) return rc;
   return sum_terms(s, workspace, loss, pairs, 1.f / (float)pairs, op);
+}
+
+int ferrite_preference_loss(void* stream, const void* logits, const void* targets, const float* ref_logp, const int64_t* offsets, float beta,
+                            float label_smoothing, int kind, int average, float temperature, float scale, float* loss, float* margins,
+                            float* logp, float* stats, float* coef, void* dlogits, float* workspace, size_t workspace_bytes, int64_t rows,
+                            int64_t pairs, int64_t vocab, int64_t ld, int64_t ld_out, int64_t ignore_index, int dtype, int target_dtype,
+                            int out_dtype) {
+  const char* op = "preference_loss";
+  if (int rc = injected_fault(op)) return rc;
+  if (dlogits) {  // before anything is launched
+    if (int rc = check_rows(op, rows, vocab, ld, temperature, dtype, ld_out, out_dtype < 0 ? 99 : out_dtype)) return rc;
+    if (rows > 0 && (!stats || !coef)) return fail(FERRITE_BAD_SHAPE, "%s: null pointer", op);
+    if (misaligned(dlogits, elem_bytes(out_dtype))) return fail(FERRITE_BAD_ALIGNMENT, "%s: misaligned pointer", op);
+  }
+  if (int rc = check_pairs(op, logp, ref_logp, targets, offsets, beta, label_smoothing, kind, loss, margins, workspace, workspace_bytes, rows, pairs, target_dtype))
+    return rc;
+  if (int rc = ferrite_logprobs_fwd(stream, logits, targets, logp, nullptr, stats, rows, vocab, ld, ignore_index, temperature, dtype, target_dtype)) return rc;
+  if (int rc = ferrite_preference_pairs(stream, logp, ref_logp, targets, offsets, beta, label_smoothing, kind, average, loss, margins, coef, workspace,
+                                        workspace_bytes, rows, pairs, ignore_index, target_dtype))
+    return rc;
+  if (!dlogits) return FERRITE_OK;
+  return ferrite_logprobs_bwd(stream, logits, targets, stats, nullptr, coef, nullptr, nullptr, scale, dlogits, rows, vocab, ld, ld_out, ignore_index,
+                              temperature, dtype, target_dtype, out_dtype);
 }
 
 }  // extern "C"

@@ -707,7 +707,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
 // --------------------------------------------------------------------------
 
 constexpr int kRingSmem = (227 - 2) * 1024 / 2 / 128 * 128;  // of each of two CTAs, besides what the system keeps
-constexpr int kMaxSlots = kHelpers * (64 + 12 * 1024);  // the helpers' lists at their longest
+constexpr int kMaxSlots = kHelpers * (2048 + 12 * 1024);  // the helpers' lists at their longest
 
 // How rows are split: chunks of each CTA's ring, log2 of the CTAs per row (-1: the row does not fit).
 // The split goes by the row's length and type alone, not by how many rows there are, with a gradient

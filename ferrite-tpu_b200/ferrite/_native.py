@@ -103,6 +103,8 @@ SIGNATURES: dict[str, tuple] = {
     "ferrite_policy_loss": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _f32, _f32, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                    _sz, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32]),
     "ferrite_preference_pairs": (_i32, [_vp, _vp, _vp, _vp, _vp, _f32, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i32]),
+    "ferrite_preference_loss": (_i32, [_vp, _vp, _vp, _vp, _vp, _f32, _f32, _i32, _i32, _f32, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64,
+                                       _i64, _i64, _i64, _i64, _i32, _i32, _i32]),
     "ferrite_distill_loss": (_i32, [_vp, _vp, _vp, _vp, _vp, _f32, _vp, _f32, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
                                     _i32, _i32, _i32]),
     "ferrite_attn_bwd_ds_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32]),
@@ -194,7 +196,7 @@ def on_tensor_device(fn):
 
     @functools.wraps(fn)
     def wrapper(*args, **kwargs):
-        for a in itertools.chain(args, kwargs.values()):
+        for a in args if args and isinstance(args[0], torch.Tensor) and args[0].is_cuda else itertools.chain(args, kwargs.values()):
             if isinstance(a, torch.Tensor) and a.is_cuda:
                 if a.device.index == torch.cuda.current_device():
                     break
@@ -210,7 +212,10 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def stream_ptr(device: torch.device | None = None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of ``device`` as the handle the library takes (without a torch.cuda.Stream
+    object made for it, which costs as much as a launch)."""
+    index = None if device is None else device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def device_status(clear: bool = True) -> None:

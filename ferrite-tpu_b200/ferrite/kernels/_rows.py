@@ -1,5 +1,8 @@
 """Argument checks and buffers that the losses over logits ``[rows, vocab]`` share
-(:mod:`ferrite.kernels.logprobs`, ``policy_loss``, ``preference_loss``, ``distillation``)."""
+(:mod:`ferrite.kernels.logprobs`, ``policy_loss``, ``preference_loss``, ``distillation``).
+
+A call on a few rows takes less time on the GPU than its checks in Python, so these look at each tensor
+once and leave a tensor that is already as the kernels want it alone."""
 
 from __future__ import annotations
 
@@ -15,14 +18,16 @@ IGNORE_INDEX = -100
 def check_logits(logits: torch.Tensor, grad_dtype=None) -> tuple[int, int]:
     """(rows, vocab) of a 2-D tensor of f32, bf16 or f16 with unit column stride, rows apart by at
     least ``vocab`` elements; ``grad_dtype`` is its own type, or a 16-bit one for f32 logits."""
-    if logits.ndim != 2:
+    if logits.dim() != 2:
         raise ValueError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
     code = nat.dtype_code(logits.dtype)
     rows, vocab = logits.shape
     if vocab < 1:
         raise ValueError("logits need at least one column")
-    if (logits.stride(1) != 1 and vocab > 1) or (rows > 1 and logits.stride(0) < vocab):
-        raise ValueError(f"logits must have unit column stride and rows that do not overlap, got strides {logits.stride()}")
+    if not logits.is_contiguous():
+        between, within = logits.stride()
+        if (within != 1 and vocab > 1) or (rows > 1 and between < vocab):
+            raise ValueError(f"logits must have unit column stride and rows that do not overlap, got strides {logits.stride()}")
     if grad_dtype is not None and grad_dtype != logits.dtype and not (code == nat.F32 and grad_dtype in (torch.bfloat16, torch.float16)):
         raise TypeError(f"gradient of type {grad_dtype} for logits of type {logits.dtype}: expected the logits' own, or 16-bit for float32")
     return rows, vocab
@@ -30,7 +35,8 @@ def check_logits(logits: torch.Tensor, grad_dtype=None) -> tuple[int, int]:
 
 def row_stride(logits: torch.Tensor) -> int:
     """The stride between rows in elements (of a single row: its length)."""
-    return logits.stride(0) if logits.shape[0] > 1 else max(logits.stride(0), logits.shape[1])
+    rows, vocab = logits.shape
+    return max(logits.stride(0), vocab) if rows > 1 else vocab
 
 
 def empty_grad(logits: torch.Tensor, dtype) -> torch.Tensor:
@@ -48,11 +54,12 @@ def empty_grad(logits: torch.Tensor, dtype) -> torch.Tensor:
 
 def check_targets(targets: torch.Tensor, rows: int) -> tuple[torch.Tensor, int]:
     """(targets as one dense row, their type's code): int32 or int64, one for each row of logits."""
-    if targets.dtype not in (torch.int32, torch.int64):
+    code = 1 if targets.dtype == torch.int64 else 0
+    if not code and targets.dtype != torch.int32:
         raise TypeError(f"targets must be int32 or int64, got {targets.dtype}")
     if targets.numel() != rows:
         raise ValueError(f"{targets.numel()} targets for {rows} rows")
-    return targets.reshape(-1).contiguous(), int(targets.dtype == torch.int64)
+    return targets if targets.is_contiguous() else targets.reshape(-1).contiguous(), code
 
 
 def per_row(t: torch.Tensor | None, rows: int, name: str) -> torch.Tensor | None:
@@ -61,6 +68,8 @@ def per_row(t: torch.Tensor | None, rows: int, name: str) -> torch.Tensor | None
         return None
     if t.numel() != rows:
         raise ValueError(f"{name}: {t.numel()} values for {rows} rows")
+    if t.dtype == torch.float32 and t.is_contiguous():
+        return t
     if not t.is_floating_point():
         raise TypeError(f"{name} must be floating point, got {t.dtype}")
     return t.detach().reshape(-1).to(torch.float32).contiguous()
@@ -78,8 +87,18 @@ def upstream(g: torch.Tensor) -> torch.Tensor:
     return g.reshape(()).to(torch.float32).contiguous()
 
 
-def same_device(logits: torch.Tensor, *others: torch.Tensor | None) -> None:
-    nat.require_cuda(logits, *others)
+def same_device(logits: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
+    """The logits' device, a GPU that the other tensors are on as well."""
+    device = logits.device
+    if not logits.is_cuda:
+        nat.require_cuda(logits)
     for t in others:
-        if t is not None and t.device != logits.device:
-            raise ValueError(f"tensors on {logits.device} and {t.device}: expected one device")
+        if t is not None and t.device != device:
+            nat.require_cuda(t)
+            raise ValueError(f"tensors on {device} and {t.device}: expected one device")
+    return device
+
+
+def differentiable(logits: torch.Tensor) -> bool:
+    """Whether a call on these logits is to be recorded."""
+    return logits.requires_grad and torch.is_grad_enabled()

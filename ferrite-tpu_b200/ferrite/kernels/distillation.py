@@ -45,18 +45,19 @@ def _check(logits, teacher_values, teacher_indices, weights, temperature, grad_d
 def _launch(logits, values, indices, weights, temperature, grad_dtype, dloss, grad_scale):
     rows, vocab = logits.shape
     top, dev = values.shape[1], logits.device
-    f = torch.empty(2 * rows + 1, dtype=torch.float32, device=dev)  # loss, per-token losses and the terms of the sum
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    f = torch.empty((2, rows), dtype=torch.float32, device=dev)  # per-token losses and the terms of the sum
     base = f.data_ptr()
     grad = None if grad_dtype is None else _rows.empty_grad(logits, grad_dtype)
     nat.check(
         nat.lib().ferrite_distill_loss(
             nat.stream_ptr(dev), logits.data_ptr(), values.data_ptr(), indices.data_ptr(), nat.ptr(weights), temperature, nat.ptr(dloss),
-            grad_scale, base, base + 4, nat.ptr(grad), base + 4 * (1 + rows), 4 * rows, rows, vocab, top, _rows.row_stride(logits),
+            grad_scale, loss.data_ptr(), base, nat.ptr(grad), base + 4 * rows, 4 * rows, rows, vocab, top, _rows.row_stride(logits),
             vocab if grad is None else _rows.row_stride(grad), top, nat.dtype_code(logits.dtype), nat.dtype_code(values.dtype), int(indices.dtype == torch.int64),
             -1 if grad_dtype is None else nat.dtype_code(grad_dtype),
         )
     )
-    return DistillationLoss(f[0], f[1 : 1 + rows]), grad
+    return DistillationLoss(loss, f.unbind()[0]), grad
 
 
 class _Distillation(torch.autograd.Function):
@@ -88,11 +89,12 @@ def distillation_loss(logits, teacher_values, teacher_indices, weights=None, *, 
     gives zeros.
     """
     values, indices, weights, temperature = _check(logits, teacher_values, teacher_indices, weights, temperature, None)
+    if not _rows.differentiable(logits):
+        return _launch(logits, values, indices, weights, temperature, None, None, 1.0)[0]
     return DistillationLoss(*_Distillation.apply(logits, values, indices, weights, temperature))
 
 
 @nat.on_tensor_device
-@torch.no_grad()
 def distillation_loss_and_grad(logits, teacher_values, teacher_indices, weights=None, *, temperature: float = 1.0, grad_scale: float = 1.0,
                                grad_dtype=None) -> tuple[DistillationLoss, torch.Tensor]:
     """:func:`distillation_loss` and ``grad_scale`` times its gradient in the logits, in one pass over

@@ -20,13 +20,13 @@ from ferrite.kernels._rows import IGNORE_INDEX
 def logprobs_forward(logits, targets, temperature: float, ignore_index: int, *, entropy: bool, stats: bool):
     """``(logp, entropy or None, stats or None)`` through ``ferrite_logprobs_fwd``; ``targets`` dense."""
     rows, vocab = logits.shape
-    f32 = {"dtype": torch.float32, "device": logits.device}
-    logp = torch.empty(rows, **f32)
-    h = torch.empty(rows, **f32) if entropy else None
-    st = torch.empty((rows, 2), **f32) if stats else None
+    dev = logits.device
+    logp = torch.empty(rows, dtype=torch.float32, device=dev)
+    h = torch.empty(rows, dtype=torch.float32, device=dev) if entropy else None
+    st = torch.empty((rows, 2), dtype=torch.float32, device=dev) if stats else None
     nat.check(
         nat.lib().ferrite_logprobs_fwd(
-            nat.stream_ptr(logits.device), logits.data_ptr(), targets.data_ptr(), logp.data_ptr(), nat.ptr(h), nat.ptr(st),
+            nat.stream_ptr(dev), logits.data_ptr(), targets.data_ptr(), logp.data_ptr(), nat.ptr(h), nat.ptr(st),
             rows, vocab, _rows.row_stride(logits), ignore_index, temperature, nat.dtype_code(logits.dtype),
             int(targets.dtype == torch.int64),
         )
@@ -51,7 +51,7 @@ def logprobs_backward(logits, targets, stats, entropy, dlogp, dentropy, dloss, s
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, temperature, entropy, ignore_index):
-        logp, h, stats = logprobs_forward(logits, targets, temperature, ignore_index, entropy=entropy, stats=logits.requires_grad)
+        logp, h, stats = logprobs_forward(logits, targets, temperature, ignore_index, entropy=entropy, stats=True)
         ctx.save_for_backward(logits, targets, stats, h)
         ctx.temperature, ctx.ignore_index = temperature, ignore_index
         return (logp, h) if entropy else logp
@@ -81,6 +81,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, temperature: 
     targets, _ = _rows.check_targets(targets, rows)
     temperature = _rows.check_temperature(temperature)
     _rows.same_device(logits, targets)
+    if not _rows.differentiable(logits):
+        logp, h, _ = logprobs_forward(logits, targets, temperature, int(ignore_index), entropy=entropy, stats=False)
+        return (logp, h) if entropy else logp
     return _TokenLogprobs.apply(logits, targets, temperature, bool(entropy), int(ignore_index))
 
 

@@ -46,21 +46,21 @@ def _launch(logits, targets, rest, clip, coefs, temperature, ignore_index, grad_
     rows, vocab = logits.shape
     old, adv, weights, ref = rest
     dev = logits.device
-    f = torch.empty(4 * rows + 1, dtype=torch.float32, device=dev)  # loss, logp, entropy, kl and the terms of the sum
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    f = torch.empty((4, rows), dtype=torch.float32, device=dev)  # logp, entropy, kl, and the terms of the sum
     base = f.data_ptr()
     clipped = torch.empty(rows, dtype=torch.bool, device=dev)
     grad = None if grad_dtype is None else _rows.empty_grad(logits, grad_dtype)
-    at = lambda i: base + 4 * (1 + i * rows)  # noqa: E731
     nat.check(
         nat.lib().ferrite_policy_loss(
             nat.stream_ptr(dev), logits.data_ptr(), targets.data_ptr(), old.data_ptr(), adv.data_ptr(), nat.ptr(weights), nat.ptr(ref),
-            clip[0], clip[1], coefs[0], coefs[1], temperature, nat.ptr(dloss), grad_scale, base, at(0), at(1), at(2),
-            clipped.data_ptr(), nat.ptr(grad), at(3), 4 * rows, rows, vocab, _rows.row_stride(logits), vocab if grad is None else _rows.row_stride(grad), ignore_index,
+            clip[0], clip[1], coefs[0], coefs[1], temperature, nat.ptr(dloss), grad_scale, loss.data_ptr(), base, base + 4 * rows,
+            base + 8 * rows, clipped.data_ptr(), nat.ptr(grad), base + 12 * rows, 4 * rows, rows, vocab, _rows.row_stride(logits), vocab if grad is None else _rows.row_stride(grad), ignore_index,
             nat.dtype_code(logits.dtype), int(targets.dtype == torch.int64), -1 if grad_dtype is None else nat.dtype_code(grad_dtype),
         )
     )
-    loss, logp, entropy, kl, _ = f.split([1, rows, rows, rows, rows])
-    return PolicyLoss(loss.view(()), logp, entropy, kl, clipped), grad
+    logp, entropy, kl, _ = f.unbind()
+    return PolicyLoss(loss, logp, entropy, kl, clipped), grad
 
 
 class _PolicyLoss(torch.autograd.Function):
@@ -93,12 +93,13 @@ def policy_loss(logits, targets, old_logprobs, advantages, weights=None, *, ref_
     ``ignore_index``, is not read and gives zeros.
     """
     targets, rest, temperature = _check(logits, targets, old_logprobs, advantages, weights, ref_logprobs, clip_low, clip_high, temperature, None)
-    return PolicyLoss(*_PolicyLoss.apply(logits, targets, rest, (float(clip_low), float(clip_high)), (float(kl_coef), float(entropy_coef)),
-                                         temperature, int(ignore_index)))
+    args = (logits, targets, rest, (float(clip_low), float(clip_high)), (float(kl_coef), float(entropy_coef)), temperature, int(ignore_index))
+    if not _rows.differentiable(logits):
+        return _launch(*args, None, None, 1.0)[0]
+    return PolicyLoss(*_PolicyLoss.apply(*args))
 
 
 @nat.on_tensor_device
-@torch.no_grad()
 def policy_loss_and_grad(logits, targets, old_logprobs, advantages, weights=None, *, ref_logprobs=None, clip_low: float = 0.2,
                          clip_high: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0, temperature: float = 1.0,
                          ignore_index: int = IGNORE_INDEX, grad_scale: float = 1.0, grad_dtype=None) -> tuple[PolicyLoss, torch.Tensor]:

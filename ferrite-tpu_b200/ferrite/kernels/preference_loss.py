@@ -24,7 +24,7 @@ import torch
 from ferrite import _native as nat
 from ferrite.kernels import _rows
 from ferrite.kernels._rows import IGNORE_INDEX
-from ferrite.kernels.logprobs import logprobs_backward, logprobs_forward
+from ferrite.kernels.logprobs import logprobs_backward
 
 KINDS = ("sigmoid", "squared", "hinge")
 
@@ -50,33 +50,43 @@ def _check(logits, targets, ref_logprobs, offsets, beta, kind, label_smoothing, 
         raise ValueError(f"beta must be positive and finite, got {beta}")
     ref = _rows.per_row(ref_logprobs, rows, "ref_logprobs")
     _rows.same_device(logits, targets, ref, offsets)
-    return targets, ref, offsets.to(torch.int64).contiguous(), _rows.check_temperature(temperature)
+    if offsets.dtype != torch.int64 or not offsets.is_contiguous():
+        offsets = offsets.to(torch.int64).contiguous()
+    return targets, ref, offsets, _rows.check_temperature(temperature)
 
 
-def _pairs(logp, ref, targets, offsets, beta, kind, label_smoothing, average, ignore_index, want_coef):
-    rows, pairs = logp.numel(), offsets.numel() // 2
-    f = torch.empty(1 + 2 * pairs + (rows if want_coef else 0), dtype=torch.float32, device=logp.device)
-    base = f.data_ptr()
+def _launch(logits, targets, ref, offsets, beta, kind, label_smoothing, average, temperature, ignore_index, keep, grad_dtype, grad_scale):
+    """``(PreferenceLoss, stats, coef, gradient)``; ``keep`` the rows' statistics and coefficients for a backward."""
+    rows, vocab = logits.shape
+    pairs, dev = offsets.numel() // 2, logits.device
+    keep = keep or grad_dtype is not None
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    per_pair = torch.empty((2, pairs), dtype=torch.float32, device=dev)  # margins and the terms of the mean
+    logp = torch.empty(rows, dtype=torch.float32, device=dev)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if keep else None
+    coef = torch.empty(rows, dtype=torch.float32, device=dev) if keep else None
+    grad = None if grad_dtype is None else _rows.empty_grad(logits, grad_dtype)
+    base = per_pair.data_ptr()
     nat.check(
-        nat.lib().ferrite_preference_pairs(
-            nat.stream_ptr(logp.device), logp.data_ptr(), ref.data_ptr(), targets.data_ptr(), offsets.data_ptr(), beta, label_smoothing,
-            KINDS.index(kind), int(average), base, base + 4, base + 4 * (1 + 2 * pairs) if want_coef else None, base + 4 * (1 + pairs),
-            4 * pairs, rows, pairs, ignore_index, int(targets.dtype == torch.int64),
+        nat.lib().ferrite_preference_loss(
+            nat.stream_ptr(dev), logits.data_ptr(), targets.data_ptr(), ref.data_ptr(), offsets.data_ptr(), beta, label_smoothing,
+            KINDS.index(kind), int(average), temperature, grad_scale, loss.data_ptr(), base, logp.data_ptr(), nat.ptr(stats), nat.ptr(coef),
+            nat.ptr(grad), base + 4 * pairs, 4 * pairs, rows, pairs, vocab, _rows.row_stride(logits),
+            vocab if grad is None else _rows.row_stride(grad), ignore_index, nat.dtype_code(logits.dtype), int(targets.dtype == torch.int64),
+            -1 if grad is None else nat.dtype_code(grad_dtype),
         )
     )
-    return f[0], f[1 : 1 + pairs], f[1 + 2 * pairs :] if want_coef else None
+    return PreferenceLoss(loss, per_pair.unbind()[0], logp), stats, coef, grad
 
 
 class _Preference(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, ref, offsets, beta, kind, label_smoothing, average, temperature, ignore_index):
-        need = logits.requires_grad
-        logp, _, stats = logprobs_forward(logits, targets, temperature, ignore_index, entropy=False, stats=need)
-        loss, margins, coef = _pairs(logp, ref, targets, offsets, beta, kind, label_smoothing, average, ignore_index, need)
+        out, stats, coef, _ = _launch(logits, targets, ref, offsets, beta, kind, label_smoothing, average, temperature, ignore_index, True, None, 1.0)
         ctx.save_for_backward(logits, targets, stats, coef)
         ctx.temperature, ctx.ignore_index = temperature, ignore_index
-        ctx.mark_non_differentiable(margins, logp)
-        return loss, margins, logp
+        ctx.mark_non_differentiable(*out[1:])
+        return tuple(out)
 
     @staticmethod
     @nat.on_tensor_device
@@ -98,12 +108,13 @@ def preference_loss(logits, targets, ref_logprobs, offsets, *, beta: float = 0.1
     no gradient.  label_smoothing is the sigmoid loss's; the others do not use it.
     """
     targets, ref, offsets, temperature = _check(logits, targets, ref_logprobs, offsets, beta, kind, label_smoothing, temperature, None)
-    return PreferenceLoss(*_Preference.apply(logits, targets, ref, offsets, float(beta), kind, float(label_smoothing), bool(average),
-                                             temperature, int(ignore_index)))
+    args = (logits, targets, ref, offsets, float(beta), kind, float(label_smoothing), bool(average), temperature, int(ignore_index))
+    if not _rows.differentiable(logits):
+        return _launch(*args, False, None, 1.0)[0]
+    return PreferenceLoss(*_Preference.apply(*args))
 
 
 @nat.on_tensor_device
-@torch.no_grad()
 def preference_loss_and_grad(logits, targets, ref_logprobs, offsets, *, beta: float = 0.1, kind: str = "sigmoid", label_smoothing: float = 0.0,
                              average: bool = False, temperature: float = 1.0, ignore_index: int = IGNORE_INDEX, grad_scale: float = 1.0,
                              grad_dtype=None) -> tuple[PreferenceLoss, torch.Tensor]:
@@ -111,10 +122,9 @@ def preference_loss_and_grad(logits, targets, ref_logprobs, offsets, *, beta: fl
     defaults to the logits' type (f32 logits also give bf16 or f16)."""
     grad_dtype = grad_dtype or logits.dtype
     targets, ref, offsets, temperature = _check(logits, targets, ref_logprobs, offsets, beta, kind, label_smoothing, temperature, grad_dtype)
-    logp, _, stats = logprobs_forward(logits, targets, temperature, ignore_index, entropy=False, stats=True)
-    loss, margins, coef = _pairs(logp, ref, targets, offsets, float(beta), kind, float(label_smoothing), average, ignore_index, True)
-    grad = logprobs_backward(logits, targets, stats, None, coef, None, None, float(grad_scale), temperature, ignore_index, grad_dtype)
-    return PreferenceLoss(loss, margins, logp), grad
+    out, _, _, grad = _launch(logits, targets, ref, offsets, float(beta), kind, float(label_smoothing), average, temperature, int(ignore_index),
+                              True, grad_dtype, float(grad_scale))
+    return out, grad
 
 
 def preference_loss_reference(logits, targets, ref_logprobs, offsets, *, beta=0.1, kind="sigmoid", label_smoothing=0.0, average=False,

@@ -317,6 +317,17 @@ FERRITE_API int ferrite_preference_pairs(void* stream, const float* logp, const 
                         float* coef, float* workspace, size_t workspace_bytes, int64_t rows,
                         int64_t pairs, int64_t ignore_index, int target_dtype);
 
+/* The preference loss from the logits: ferrite_logprobs_fwd, ferrite_preference_pairs and, when
+ * dlogits is given, ferrite_logprobs_bwd of its coef (times scale), in one call.  logp, coef: rows
+ * floats; stats: 2 rows floats (8-byte aligned); coef and stats may be NULL without dlogits. */
+FERRITE_API int ferrite_preference_loss(void* stream, const void* logits, const void* targets,
+                        const float* ref_logp, const int64_t* offsets, float beta,
+                        float label_smoothing, int kind, int average, float temperature, float scale,
+                        float* loss, float* margins, float* logp, float* stats, float* coef,
+                        void* dlogits, float* workspace, size_t workspace_bytes, int64_t rows,
+                        int64_t pairs, int64_t vocab, int64_t ld, int64_t ld_out,
+                        int64_t ignore_index, int dtype, int target_dtype, int out_dtype);
+
 /* Distillation from a teacher's top logits, and in the same pass its gradient when
  * dlogits is given: values (value_dtype) and indices (index_dtype 0 int32, 1 int64) are
  * [rows, top] lists with row stride ld_list, 1 <= top <= 1024.
