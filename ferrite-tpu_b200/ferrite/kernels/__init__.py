@@ -5,6 +5,7 @@ from ferrite.kernels.matmul import matmul, matmul_reference
 from ferrite.kernels.policy_loss import policy_loss, policy_loss_and_grad, policy_loss_reference
 from ferrite.kernels.preference_loss import preference_loss, preference_loss_and_grad, preference_loss_reference
 from ferrite.kernels.rmsnorm import rmsnorm, rmsnorm_reference
+from ferrite.kernels.tied_head import tied_head_distillation_loss, tied_head_policy_loss, tied_head_preference_loss
 
 __all__ = [
     "distillation_loss",
@@ -22,6 +23,9 @@ __all__ = [
     "preference_loss_reference",
     "rmsnorm",
     "rmsnorm_reference",
+    "tied_head_distillation_loss",
+    "tied_head_policy_loss",
+    "tied_head_preference_loss",
     "token_logprobs",
     "token_logprobs_reference",
 ]
