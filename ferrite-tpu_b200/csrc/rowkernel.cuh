@@ -363,7 +363,11 @@ struct LiveRows {
 struct Place {
   int at = 0;
   uint32_t parity = 0;
-  __device__ __forceinline__ void next(int size, int n = 1) {  // n <= size
+  __device__ __forceinline__ void next(int size, int n = 1) {
+    while (n > size) {
+      n -= size;
+      parity ^= 1;
+    }
     at += n;
     if (at >= size) {
       at -= size;
@@ -373,7 +377,7 @@ struct Place {
 };
 
 template <class Op, typename TI, typename TO, bool GRAD>
-__global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut out, Op op, int ring_chunks, int lg_cluster) {
+__global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut out, Op op, int ring_chunks, int lg_cluster, int twice) {
   constexpr int N = 16 / sizeof(TI);
   constexpr bool kSums = !Op::kHasStats;        // a first pass
   constexpr bool kBoth = GRAD && kSums;         // both passes
@@ -425,6 +429,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
       if (!rows.next(r)) continue;
       const TI* x = static_cast<const TI*>(in.logits) + r * in.ld;
       sl.at(x);
+      for (int pass = 0; pass <= (kBoth ? twice : 0); ++pass) {
       const int c0 = (group - k + kGroups) % kGroups;
       Place at = p;
       at.next(ring_chunks, c0);
@@ -447,6 +452,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
         at.next(ring_chunks, kGroups);
         src += kGroups * kChunk;
         left -= kGroups * kChunkVec;
+      }
       }
     }
     // the last copy into each chunk has landed before the CTA gives up its shared memory
@@ -552,7 +558,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
         int left = sl.nv - c0 * kChunkVec - gtid;
         TO* to = dx + col0 + (c0 * kChunkVec + gtid) * N;
         for (int c = c0; c < sl.chunks; c += kGroups) {
-          if constexpr (!kSums) (void)mbar_wait(&sh.full[at.at], at.parity, abort, 208);
+          if (!kSums || twice) (void)mbar_wait(&sh.full[at.at], at.parity, abort, 208);
           const uint4* p = reinterpret_cast<const uint4*>(ring + (size_t)at.at * kChunk) + gtid;
           if constexpr (kUsual) {  // all of the thread's vectors, side by side
             uint4 raw[kVecPer];
@@ -658,7 +664,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
               push<Op::kEnt>(st, nc, vals, in, kk);
             }
         }
-        if constexpr (!kBoth) {
+        if (!kBoth || twice) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.empty[at.at]);
         }
@@ -695,7 +701,17 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
         continue;
       }
       if constexpr (kSums) first(r);
-      if constexpr (GRAD) second(r);
+      if constexpr (GRAD) {
+        if (kSums && twice) {
+          p2 = p1;
+          k2 = k1;
+        }
+        second(r);
+        if (kSums && twice) {
+          p1 = p2;
+          k1 = k2;
+        }
+      }
     }
   }
   __syncwarp();
@@ -714,7 +730,7 @@ constexpr int kMaxSlots = kHelpers * (2048 + 12 * 1024);  // the helpers' lists 
 // or without: so a row's results have the same bits in every call (log-probabilities taken in one
 // batch and compared in another differ by nothing), as long as it starts on a 16-byte boundary.
 struct RingPlan {
-  int chunks, lg_cluster;
+  int chunks, lg_cluster, twice;
   size_t smem;
 };
 inline RingPlan plan_ring(int64_t vocab, int elem, int slot_bytes) {
@@ -730,6 +746,7 @@ inline RingPlan plan_ring(int64_t vocab, int elem, int slot_bytes) {
   int lg = 0;
   while ((1 << lg) < kRingCluster && ((bytes + 15) >> lg) + 16 > most) ++lg;
   p.lg_cluster = ((bytes + 15) >> lg) + 16 > most ? -1 : lg;
+  if (lg > 0) p.twice = 1, p.lg_cluster = 0;
   return p;
 }
 
@@ -761,7 +778,7 @@ static int launch_row(cudaStream_t s, const RowIn& in, const RowOut& out, const 
     }
     const int64_t used = in.rows < clusters ? in.rows : clusters;
     e = launch_pdl_cluster(kern, dim3((unsigned)(used << p.lg_cluster)), dim3(kRingThreads), p.smem, s, 1u << p.lg_cluster, in, out, op,
-                           p.chunks, p.lg_cluster);
+                           p.chunks, p.lg_cluster, p.twice);
   } else {
     e = launch_pdl(row_kernel<Op, TI, TO, GRAD>, dim3((unsigned)in.rows), dim3(row_threads(in.vocab)), op.slot_bytes(), s, in, out, op);
   }
