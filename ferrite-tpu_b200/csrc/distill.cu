@@ -92,18 +92,34 @@ struct Distill {
     const int lane = threadIdx.x & 31;
     float m = -INFINITY, bad = 0.f, first = -INFINITY;
     int count = 0;
-    for (int j = lane; j < top; j += 32) {
-      int64_t i = index(r * ld_list + j);
-      const float v = value(r * ld_list + j);
-      if (v == -INFINITY) i = -1;
-      if (i >= in.vocab) bad = __int_as_float(0x7fc00000), i = -1;
-      l.idx[j] = i < 0 ? -1 : (int)i;
-      l.x[j] = i < 0 ? 0.f : DT<TI>::to_f(x[i]);
-      l.q[j] = v;
-      if (i >= 0) {
-        if (count == 0) first = l.x[j];
-        ++count;
-        m = fmaxf(m, v);  // a NaN value shows through the sums
+    // Four entries a lane at a time: their tokens and values are all asked for before the first logit.
+    for (int j0 = lane; j0 < top; j0 += 128) {
+      int64_t i[4];
+      float v[4], xs[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int j = j0 + 32 * q;
+        i[q] = j < top ? index(r * ld_list + j) : -1;
+        v[q] = j < top ? value(r * ld_list + j) : -INFINITY;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (v[q] == -INFINITY) i[q] = -1;
+        if (i[q] >= in.vocab) bad = __int_as_float(0x7fc00000), i[q] = -1;
+        xs[q] = i[q] < 0 ? 0.f : DT<TI>::to_f(x[i[q]]);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int j = j0 + 32 * q;
+        if (j >= top) break;
+        l.idx[j] = i[q] < 0 ? -1 : (int)i[q];
+        l.x[j] = xs[q];
+        l.q[j] = v[q];
+        if (i[q] >= 0) {
+          if (count == 0) first = xs[q];
+          ++count;
+          m = fmaxf(m, v[q]);  // a NaN value shows through the sums
+        }
       }
     }
 #pragma unroll
@@ -139,25 +155,10 @@ struct Distill {
     }
     return base_of(first, in);
   }
-  __device__ Coef finish(int64_t r, const Norm& w, const RowIn& in, float g, bool writer, char* slot) const {
-    const List l = list(slot);
+  __device__ Coef finish(int64_t, const Norm& w, const RowIn& in, float g, char* slot) const {
     const Row& row = *reinterpret_cast<const Row*>(slot);
     Coef cf;
     const float scale = grad_base(w, in, cf) / w.s;
-    if (writer) {
-      const int lane = threadIdx.x & 31;
-      const float ls = log2f(w.s);
-      float part = 0.f;
-      for (int j = lane; j < top; j += 32)
-        if (l.idx[j] >= 0 && l.q[j] != 0.f) part += l.q[j] * (y_of(l.x[j], w, in) - ls);
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) part += __shfl_xor_sync(0xffffffffu, part, off);
-      if (lane == 0) {
-        const float per = row.entries ? tau * tau * kLn2 * (row.qlogq - part) + row.bad : 0.f;
-        per_token[r] = per;
-        terms[r] = row.entries ? row.w * per : 0.f;
-      }
-    }
     const float f = row.w * tau * g + row.bad;
     cf.A = f * scale;
     cf.B = 0.f;
@@ -166,15 +167,31 @@ struct Distill {
     cf.masked = row.entries == 0;
     return cf;
   }
-  // The listed tokens' entries in [lo, hi), by threads tid < threads.  Where a token is listed twice, the
+  __device__ void results(int64_t r, const Norm& w, const RowIn& in, char* slot) const {
+    const List l = list(slot);
+    const Row& row = *reinterpret_cast<const Row*>(slot);
+    const int lane = threadIdx.x & 31;
+    const float ls = log2f(w.s);
+    float part = 0.f;
+    for (int j = lane; j < top; j += 32)
+      if (l.idx[j] >= 0 && l.q[j] != 0.f) part += l.q[j] * (y_of(l.x[j], w, in) - ls);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) part += __shfl_xor_sync(0xffffffffu, part, off);
+    if (lane == 0) {
+      const float per = row.entries ? tau * tau * kLn2 * (row.qlogq - part) + row.bad : 0.f;
+      per_token[r] = per;
+      terms[r] = row.entries ? row.w * per : 0.f;
+    }
+  }
+  // The listed tokens' entries, by threads tid < threads.  Where a token is listed twice, the
   // thread of each of its entries sums all their weights, and writes the same value.
   template <typename TO>
-  __device__ void fix(const Coef& cf, TO* dx, int lo, int hi, const RowIn& in, char* slot, int tid, int threads) const {
+  __device__ void fix(const Coef& cf, TO* dx, const RowIn& in, char* slot, int tid, int threads) const {
     const List l = list(slot);
     const bool twice = reinterpret_cast<const Row*>(slot)->twice;
     for (int j = tid; j < top; j += threads) {
       const int i = l.idx[j];
-      if (i < lo || i >= hi) continue;  // absent entries too: lo is not negative
+      if (i < 0) continue;  // absent
       float q = l.q[j];
       if (twice) {
         q = 0.f;

@@ -45,13 +45,13 @@ struct LogprobsFwd {
     if ((threadIdx.x & 31) == 0) reinterpret_cast<Row*>(slot)->xt = xt;
     return base_of(xt, in);
   }
-  __device__ Coef finish(int64_t r, const Norm& w, const RowIn& in, float, bool writer, char* slot) const {
-    if (writer && (threadIdx.x & 31) == 0) {
+  __device__ Coef finish(int64_t, const Norm&, const RowIn&, float, char*) const { return Coef{}; }
+  __device__ void results(int64_t r, const Norm& w, const RowIn& in, char* slot) const {
+    if ((threadIdx.x & 31) == 0) {
       logp[r] = logp_of(reinterpret_cast<Row*>(slot)->xt, w, in);
       if constexpr (ENT) entropy[r] = entropy_of(w);
       if (stats) stats[r] = make_float2(w.base, w.big ? -w.s : w.s);
     }
-    return Coef{};
   }
 };
 
@@ -92,10 +92,11 @@ struct LogprobsBwd {
     return 0.f;
   }
   __device__ Norm state(const char* slot) const { return reinterpret_cast<const Row*>(slot)->w; }
-  __device__ Coef finish(int64_t, const Norm& w, const RowIn& in, float g, bool, char* slot) const {
+  __device__ Coef finish(int64_t, const Norm& w, const RowIn& in, float g, char* slot) const {
     const Row& row = *reinterpret_cast<const Row*>(slot);
     return coef_of<ENT>(row.a, row.b, g, row.t, row.xt, w, in);
   }
+  __device__ void results(int64_t, const Norm&, const RowIn&, char*) const {}
 };
 
 // ENT: the entropy bonus takes part in the gradient (its value is always written).
@@ -134,28 +135,37 @@ struct Policy {
     if ((threadIdx.x & 31) == 0) *reinterpret_cast<Row*>(slot) = Row{p.t, p.w, xt, old_logp[r], adv[r], ref ? ref[r] : 0.f};
     return base_of(xt, in);
   }
-  __device__ Coef finish(int64_t r, const Norm& w, const RowIn& in, float g, bool writer, char* slot) const {
-    const Row row = *reinterpret_cast<const Row*>(slot);
-    const float lp = logp_of(row.xt, w, in), h = entropy_of(w);
-    const float ratio = expf(lp - row.old_logp);
-    const float plain = ratio * row.adv, bounded = fminf(fmaxf(ratio, 1.f - lo), 1.f + hi) * row.adv;
-    const bool cut = bounded < plain;
-    float per = cut ? -bounded : -plain, da = cut ? 0.f : -plain, klv = 0.f;
-    if (ref) {
-      const float d = row.ref - lp, em = expm1f(d);
-      klv = em - d;
-      per = fmaf(beta, klv, per);
-      da = fmaf(-beta, em, da);
-    }
-    per = fmaf(-ent_coef, h, per);
-    if (writer && (threadIdx.x & 31) == 0) {
-      terms[r] = row.w * per;
-      logp[r] = lp;
+  struct Step {
+    float logp, ratio, plain, bounded, em;  // em = exp(ref - logp) - 1
+    bool cut;
+  };
+  __device__ Step step(const Row& row, const Norm& w, const RowIn& in) const {
+    Step t;
+    t.logp = logp_of(row.xt, w, in);
+    t.ratio = expf(t.logp - row.old_logp);
+    t.plain = t.ratio * row.adv;
+    t.bounded = fminf(fmaxf(t.ratio, 1.f - lo), 1.f + hi) * row.adv;
+    t.cut = t.bounded < t.plain;
+    t.em = ref ? expm1f(row.ref - t.logp) : 0.f;
+    return t;
+  }
+  __device__ Coef finish(int64_t, const Norm& w, const RowIn& in, float g, char* slot) const {
+    const Row& row = *reinterpret_cast<const Row*>(slot);
+    const Step t = step(row, w, in);
+    const float da = fmaf(-beta, t.em, t.cut ? 0.f : -t.plain);
+    return coef_of<ENT>(row.w * da, ENT ? -row.w * ent_coef : 0.f, g, row.t, row.xt, w, in);
+  }
+  __device__ void results(int64_t r, const Norm& w, const RowIn& in, char* slot) const {
+    const Row& row = *reinterpret_cast<const Row*>(slot);
+    const Step t = step(row, w, in);
+    const float h = entropy_of(w), klv = ref ? t.em - (row.ref - t.logp) : 0.f;
+    if ((threadIdx.x & 31) == 0) {
+      terms[r] = row.w * fmaf(-ent_coef, h, fmaf(beta, klv, t.cut ? -t.bounded : -t.plain));
+      logp[r] = t.logp;
       entropy[r] = h;
       kl[r] = klv;
-      clipped[r] = cut;
+      clipped[r] = t.cut;
     }
-    return coef_of<ENT>(row.w * da, ENT ? -row.w * ent_coef : 0.f, g, row.t, row.xt, w, in);
   }
 };
 
