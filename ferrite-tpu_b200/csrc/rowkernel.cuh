@@ -49,14 +49,44 @@ __device__ __forceinline__ void store_at(TO* p, const float (&d)[N], bool vec) {
   }
 }
 
+// What stands for the elements of vectors past a row's end: nothing of the sums.  -inf, but in 0 * y
+// where the entropy is summed -1e30; f16 has none that is small enough for every temperature.
+template <typename T, bool ENT>
+struct Pad {
+  static constexpr bool kThere = !ENT || !std::is_same_v<T, __half>;
+  static constexpr uint32_t kBits = std::is_same_v<T, float>    ? (ENT ? 0xf149f2cau : 0xff800000u)
+                                    : std::is_same_v<T, __half> ? 0xfc00fc00u
+                                                                : (ENT ? 0xf149f149u : 0xff80ff80u);
+  static __device__ __forceinline__ uint4 vector() { return make_uint4(kBits, kBits, kBits, kBits); }
+};
+// Adds Q vectors to a state by one check of their sums; false, and nothing added, if they are not usual.
+template <bool ENT, typename T, int Q>
+__device__ __forceinline__ bool push_usual(State& st, float nc, const uint4 (&raw)[Q], const Pairs2& kk) {
+  uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    float vals[16 / sizeof(T)];
+    unpack16<T>(raw[q], vals);
+    sum_usual<ENT>(s2, u2, vals, nc, kk);
+  }
+  const float s = f2_lo(s2) + f2_hi(s2), u = ENT ? f2_lo(u2) + f2_hi(u2) : 0.f;
+  if (!usual<ENT>(s, u)) return false;
+  st.s += s;
+  if constexpr (ENT) st.u += u;
+  return true;
+}
+
 // --------------------------------------------------------------------------
-// Short rows: a warp per row, which reads it twice (the second time from L1).  No barriers; many rows
-// in flight hide the latency of each.
+// Short rows: a warp per row, which reads it twice (the second time from L1 or L2).  No barriers; many
+// rows in flight hide the latency of each.  Bound by that latency and by the work of a row that does
+// not grow with it.  At 16 KB the other kernel's stream of copies wins (policy, 16384 x 8192 bf16: 171 us
+// against 195; half as long rows 158 against 89).
 // --------------------------------------------------------------------------
 
 constexpr int kShortWarps = 4;                 // rows of a CTA
 constexpr int kShortSlots = 48 * 1024;         // shared memory that their ops may take
-constexpr int kShortRow = 8192;                // bytes: longer rows go to the kernels for whole CTAs
+constexpr int kShortVecs = 4;                  // vectors a lane asks for at a time
+constexpr int kShortRow = 16384;               // bytes: rows from this on go to the kernel for whole CTAs
 
 template <class Op, typename TI, typename TO, bool GRAD>
 __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, RowOut out, Op op) {
@@ -97,10 +127,26 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
       w = op.state(slot);
     } else {
       float nc = minus_c(st.m, in);
-      for (int v = lane; v < cut.nv; v += 32) {
-        float vals[N];
-        unpack16<TI>(ld_v4(x + cut.head + v * N), vals);
-        push<Op::kEnt>(st, nc, vals, in, kk);
+      using P = Pad<TI, Op::kEnt>;
+      for (int v = lane; v < cut.nv; v += 32 * kShortVecs) {
+        const TI* at = x + cut.head + v * N;
+        const int left = cut.nv - v;
+        uint4 raw[kShortVecs];
+        bool by_one = !P::kThere && (kShortVecs - 1) * 32 >= left;
+        if (!by_one) {
+#pragma unroll
+          for (int q = 0; q < kShortVecs; ++q) raw[q] = q * 32 < left ? ld_v4(at + q * 32 * N) : P::vector();
+          by_one = !push_usual<Op::kEnt, TI>(st, nc, raw, kk);
+        }
+        if (by_one) {
+#pragma unroll 1
+          for (int q = 0; q < kShortVecs; ++q)
+            if (q * 32 < left) {
+              float vals[N];
+              unpack16<TI>(ld_v4(at + q * 32 * N), vals);
+              push<Op::kEnt>(st, nc, vals, in, kk);
+            }
+        }
       }
       if (edge >= 0) {
         const float one[1] = {edge_x};
@@ -116,15 +162,34 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
         zeros();
         continue;
       }
-      for (int v = lane; v < cut.nv; v += 32) {
-        const int i = cut.head + v * N;
-        float vals[N], d[N];
-        unpack16<TI>(ld_v4(x + i), vals);
-        if (cf.big) grads_of<Op::kGradEnt, true>(vals, d, in.k, cf, kk);
-        else grads_of<Op::kGradEnt, false>(vals, d, in.k, cf, kk);
-        store_at(dx + i, d, vec);
-        if ((unsigned)(cf.t - i) < (unsigned)N) dx[cf.t] = DT<TO>::from_f(cf.at_t);
+      if (vec && !cf.big) {
+        for (int v = lane; v < cut.nv; v += 32 * kShortVecs) {
+          const int i = cut.head + v * N, left = cut.nv - v;
+          uint4 raw[kShortVecs];
+#pragma unroll
+          for (int q = 0; q < kShortVecs; ++q)
+            if (q * 32 < left) raw[q] = ld_v4(x + i + q * 32 * N);
+#pragma unroll
+          for (int q = 0; q < kShortVecs; ++q) {
+            float vals[N], d[N];
+            unpack16<TI>(raw[q], vals);
+            grads_of<Op::kGradEnt, false>(vals, d, in.k, cf, kk);
+            if (q * 32 < left) store_vec<TO, N>(dx + i + q * 32 * N, d);
+          }
+        }
+      } else {
+        for (int v = lane; v < cut.nv; v += 32) {
+          const int i = cut.head + v * N;
+          float vals[N], d[N];
+          unpack16<TI>(ld_v4(x + i), vals);
+          if (cf.big) grads_of<Op::kGradEnt, true>(vals, d, in.k, cf, kk);
+          else grads_of<Op::kGradEnt, false>(vals, d, in.k, cf, kk);
+          store_at(dx + i, d, vec);
+        }
       }
+      // the target's entry, by the lane that has stored the vector it lies in
+      const int tv = (cf.t - cut.head) / N;
+      if (cf.t >= cut.head && tv < cut.nv && tv % 32 == lane) dx[cf.t] = DT<TO>::from_f(cf.at_t);
       if (edge >= 0) dx[edge] = DT<TO>::from_f(edge == cf.t ? cf.at_t : grad_of<Op::kGradEnt>(edge_x, in.k, cf));
       if constexpr (Op::kList) {
         __syncwarp();  // the entries below overwrite what another lane has stored
@@ -135,7 +200,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
 }
 
 // --------------------------------------------------------------------------
-// Rows of 8 KB and more: one read from HBM, one write.
+// Rows of 16 KB and more: one read from HBM, one write.
 //
 // Bound: HBM.  Both passes over a row (the sums, then the gradient) stream it through shared memory,
 // the second one from L2, where the rows in flight stay (296 CTAs x 125 KB are 37 MB): the first
@@ -441,12 +506,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
       (void)mbar_wait(&sh.ready[slot1.at], slot1.parity, abort, 211);
       State st = empty_state(sh.base[slot1.at]);
       float nc = minus_c(st.m, in);
-      // What stands for the elements past the row's end in its last chunk: nothing of the sums.  -inf,
-      // but in 0 * y where the entropy is summed -1e30; f16 has none that is small enough for every
-      // temperature, and sums such a chunk vector by vector.
-      constexpr bool kPad = !Op::kEnt || !std::is_same_v<TI, __half>;
-      const uint32_t pad = std::is_same_v<TI, float> ? (Op::kEnt ? 0xf149f2cau : 0xff800000u)
-                           : std::is_same_v<TI, __half> ? 0xfc00fc00u : (Op::kEnt ? 0xf149f149u : 0xff80ff80u);
+      using P = Pad<TI, Op::kEnt>;
       Place at;
       const int c0 = enter(at);
       int left = row.nv - c0 * kChunkVec - gtid;
@@ -454,26 +514,14 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
         (void)mbar_wait(&sh.full[at.at], at.parity, abort, 209);
         const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)at.at * kChunk) + gtid;
         bool by_one = true;
-        if (kPad || (kVecPer - 1) * kGroup < left) {  // all of the thread's vectors at once, one check for them
+        if (P::kThere || (kVecPer - 1) * kGroup < left) {  // all of the thread's vectors at once
           uint4 raw[kVecPer];
 #pragma unroll
           for (int q = 0; q < kVecPer; ++q) {
             raw[q] = v[q * kGroup];  // past the row's end: whatever the chunk holds
-            if (kPad && q * kGroup >= left) raw[q] = make_uint4(pad, pad, pad, pad);
+            if (P::kThere && q * kGroup >= left) raw[q] = P::vector();
           }
-          uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
-#pragma unroll
-          for (int q = 0; q < kVecPer; ++q) {
-            float vals[N];
-            unpack16<TI>(raw[q], vals);
-            sum_usual<Op::kEnt>(s2, u2, vals, nc, kk);
-          }
-          const float s = f2_lo(s2) + f2_hi(s2), u = Op::kEnt ? f2_lo(u2) + f2_hi(u2) : 0.f;
-          if (usual<Op::kEnt>(s, u)) {
-            st.s += s;
-            if constexpr (Op::kEnt) st.u += u;
-            by_one = false;
-          }
+          by_one = !push_usual<Op::kEnt, TI>(st, nc, raw, kk);
         }
         if (by_one) {
 #pragma unroll 1
