@@ -188,8 +188,8 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
         }
       }
       // the target's entry, by the lane that has stored the vector it lies in
-      const int tv = (cf.t - cut.head) / N;
-      if (cf.t >= cut.head && tv < cut.nv && tv % 32 == lane) dx[cf.t] = DT<TO>::from_f(cf.at_t);
+      const uint32_t tv = (uint32_t)(cf.t - cut.head) / N;  // not a vector of the row where t < head
+      if (tv < (uint32_t)cut.nv && tv % 32 == lane) dx[cf.t] = DT<TO>::from_f(cf.at_t);
       if (edge >= 0) dx[edge] = DT<TO>::from_f(edge == cf.t ? cf.at_t : grad_of<Op::kGradEnt>(edge_x, in.k, cf));
       if constexpr (Op::kList) {
         __syncwarp();  // the entries below overwrite what another lane has stored
@@ -304,12 +304,13 @@ template <class Op>
 struct LiveRows {
   const Op& op;
   int64_t rows, step;
+  bool backwards;  // row r stands for rows - 1 - r
   uint32_t mask = 0;
   int left = 0;
   __device__ __forceinline__ bool next(int64_t r) {
     if (left == 0) {
       const int64_t q = r + (int64_t)(threadIdx.x & 31) * step;
-      mask = __ballot_sync(0xffffffffu, q < rows && op.live(op.pre(q)));
+      mask = __ballot_sync(0xffffffffu, q < rows && op.live(op.pre(backwards ? rows - 1 - q : q)));
       left = 32;
     }
     const bool live = mask & 1u;
@@ -344,7 +345,10 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
   char* slots = ring + (size_t)ring_chunks * kChunk;
   volatile int* abort = &sh.abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // With statistics from an earlier pass over the same rows, the last rows come first: they are what
+  // that pass has left in L2.
   const int64_t step = gridDim.x, r0 = blockIdx.x;
+  auto nth = [&](int64_t r) { return Op::kHasStats ? in.rows - 1 - r : r; };
   if (tid == 0) {
     for (int i = 0; i < ring_chunks; ++i) {
       mbar_init(&sh.full[i], 1);
@@ -363,7 +367,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
   __syncthreads();
   pdl_wait();
 
-  LiveRows<Op> rows{op, in.rows, step};
+  LiveRows<Op> rows{op, in.rows, step, Op::kHasStats};
   Chunks<TI> row((int)in.vocab);
   // registers go where the passes need them: 256 x 88 + 128 x 64 = 384 x 80 of the launch
   if (warp >= kWarps) {
@@ -406,9 +410,9 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
       for (int64_t r = r0;; r += step) {  // the order of the passes below
         while (r < in.rows && !rows.next(r)) r += step;
         const bool more = r < in.rows;
-        if (kSums && more) copy(r, !GRAD);
+        if (kSums && more) copy(nth(r), !GRAD);
         const int64_t due = kSums && lag ? behind : more ? r : -1;
-        if (GRAD && due >= 0) copy(due, true);
+        if (GRAD && due >= 0) copy(nth(due), true);
         if (!more) break;
         behind = r;
       }
@@ -441,7 +445,8 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
       };
       // Fetches row r into one of the helper's two slots and announces its base.
       auto fetch = [&](int which) {
-        const float base = op.prep(r, op.pre(r), static_cast<const TI*>(in.logits) + r * in.ld, in, slots + (2 * h + which) * slot_bytes);
+        const int64_t at = nth(r);
+        const float base = op.prep(at, op.pre(at), static_cast<const TI*>(in.logits) + at * in.ld, in, slots + (2 * h + which) * slot_bytes);
         __syncwarp();
         if (kSums && lane == 0) {
           sh.base[h] = base;
@@ -451,13 +456,14 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
       next_row();
       if (r < in.rows) fetch(0);
       while (r < in.rows) {
-        const int64_t now = r;
+        const int64_t now = nth(r);
         char* slot = slots + (2 * h + parity) * slot_bytes;
         Norm w;
         if constexpr (kSums) {
           (void)wait_idle(&sh.states[h], parity, abort, 203);
           __syncwarp();
-          w = normalise<Op::kEnt>(warp_merge<Op::kEnt>(lane < kWarps ? sh.warp_state[h][lane] : empty_state(sh.warp_state[h][0].m), in), in);
+          const State st = lane < kWarps ? sh.warp_state[h][lane] : empty_state(sh.warp_state[h][0].m);
+          w = normalise<Op::kEnt>(warp_merge<Op::kEnt>(st, in), in);
         } else {
           w = op.state(slot);
           // the passes have read the coefficients of this helper's row before
@@ -485,12 +491,12 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
   } else {  // ---- the passes
     setmaxnreg_inc<88>();
     const Pairs2 kk(in);
-    const int group = warp / (kGroup / 32), gtid = tid % kGroup;
+    const uint32_t group = warp / (kGroup / 32), gtid = tid % kGroup;
     Place p, slot1, slot2;  // of the next pass's first chunk; of the helpers of the first and the second pass
-    int k = 0;              // which group has that chunk
+    uint32_t k = 0;         // which group has that chunk
     // This group's first chunk of a pass over `row`, after which p and k are the next pass's.
     auto enter = [&](Place& at) {
-      const int c0 = (group - k + kGroups) % kGroups;
+      const int c0 = (int)((group - k + kGroups) % kGroups);
       at = p;
       at.next(ring_chunks, c0);
       p.next(ring_chunks, row.chunks);
@@ -509,7 +515,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
       using P = Pad<TI, Op::kEnt>;
       Place at;
       const int c0 = enter(at);
-      int left = row.nv - c0 * kChunkVec - gtid;
+      int left = row.nv - c0 * kChunkVec - (int)gtid;
       for (int c = c0; c < row.chunks; c += kGroups) {
         (void)mbar_wait(&sh.full[at.at], at.parity, abort, 209);
         const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)at.at * kChunk) + gtid;
@@ -561,15 +567,15 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
       const float edge_x = edge >= 0 ? DT<TI>::to_f(x[edge]) : 0.f;
       (void)mbar_wait(&sh.done[slot2.at], slot2.parity, abort, 207);
       const Coef cf = sh.coef[slot2.at];
-      const int k_row = k;
+      const uint32_t k_row = k;
       Place first_at;
       const int c0 = enter(first_at);
       // What is the same for a whole row is decided here, not vector by vector.
       auto chunks = [&](auto usual_row) {
         constexpr bool kUsual = decltype(usual_row)::value;
         Place at = first_at;
-        int left = row.nv - c0 * kChunkVec - gtid;
-        TO* to = dx + row.head + (c0 * kChunkVec + gtid) * N;
+        int left = row.nv - c0 * kChunkVec - (int)gtid;
+        TO* to = dx + row.head + (c0 * kChunkVec + (int)gtid) * N;
         for (int c = c0; c < row.chunks; c += kGroups) {
           (void)mbar_wait(&sh.full[at.at], at.parity, abort, 208);
           const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)at.at * kChunk) + gtid;
@@ -614,8 +620,8 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
       else chunks(std::false_type());
       if (edge >= 0) dx[edge] = DT<TO>::from_f(cf.masked ? 0.f : edge == cf.t ? cf.at_t : grad_of<Op::kGradEnt>(edge_x, in.k, cf));
       // the target's entry, by the thread that has stored the vector it lies in
-      const int tv = (cf.t - row.head) / N;
-      if (cf.t >= row.head && tv < row.nv && tv % kGroup == gtid && (tv / kChunkVec + k_row) % kGroups == group) dx[cf.t] = DT<TO>::from_f(cf.at_t);
+      const uint32_t tv = (uint32_t)(cf.t - row.head) / N;  // not a vector of the row where t < head
+      if (tv < (uint32_t)row.nv && tv % kGroup == gtid && (tv / kChunkVec + k_row) % kGroups == group) dx[cf.t] = DT<TO>::from_f(cf.at_t);
       if constexpr (kFix || !kSums) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.written[slot2.at]);
@@ -625,10 +631,11 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
     int64_t behind = -1;
     for (int64_t r = r0;; r += step) {
       for (; r < in.rows && !rows.next(r); r += step) {  // masked
-        if (tid == 0) op.dead(r);
+        const int64_t at = nth(r);
+        if (tid == 0) op.dead(at);
         if constexpr (GRAD) {
-          TO* dx = static_cast<TO*>(out.dlogits) + r * out.ld;
-          row.at(static_cast<const TI*>(in.logits) + r * in.ld);
+          TO* dx = static_cast<TO*>(out.dlogits) + at * out.ld;
+          row.at(static_cast<const TI*>(in.logits) + at * in.ld);
           const bool vec = vector_rows<TO, N>(dx, row.head);
           const float zero[N] = {};
           for (int v = tid; v < row.nv; v += kPass) store_at(dx + row.head + v * N, zero, vec);
@@ -641,7 +648,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
         if (more) first(r);
       if constexpr (GRAD) {
         const int64_t due = kSums && lag ? behind : more ? r : -1;
-        if (due >= 0) second(due);
+        if (due >= 0) second(nth(due));
       }
       if (!more) break;
       behind = r;

@@ -42,11 +42,13 @@ def row_stride(logits: torch.Tensor) -> int:
 def empty_grad(logits: torch.Tensor, dtype) -> torch.Tensor:
     """An uninitialised ``[rows, vocab]`` gradient, its rows apart and aligned as the logits' are (so
     that a kernel can move both in the same vectors); dense where the logits' rows lie far apart."""
+    lead = logits.data_ptr() % 16 // logits.element_size()
+    if not lead and logits.is_contiguous():
+        return torch.empty_like(logits) if dtype == logits.dtype else torch.empty_like(logits, dtype=dtype)
     rows, vocab = logits.shape
     ld = row_stride(logits)
     if ld > vocab + max(64, vocab // 16):
         ld = vocab
-    lead = logits.data_ptr() % 16 // logits.element_size()
     if ld == vocab and not lead:
         return torch.empty((rows, vocab), dtype=dtype, device=logits.device)
     return torch.empty(rows * ld + lead, dtype=dtype, device=logits.device).as_strided((rows, vocab), (ld, 1), lead)
@@ -87,16 +89,15 @@ def upstream(g: torch.Tensor) -> torch.Tensor:
     return g.reshape(()).to(torch.float32).contiguous()
 
 
-def same_device(logits: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
-    """The logits' device, a GPU that the other tensors are on as well."""
-    device = logits.device
+def same_device(logits: torch.Tensor, *others: torch.Tensor | None) -> None:
+    """Refuses tensors that are not all on one GPU."""
     if not logits.is_cuda:
         nat.require_cuda(logits)
+    index = logits.get_device()
     for t in others:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             nat.require_cuda(t)
-            raise ValueError(f"tensors on {device} and {t.device}: expected one device")
-    return device
+            raise ValueError(f"tensors on {logits.device} and {t.device}: expected one device")
 
 
 def differentiable(logits: torch.Tensor) -> bool:

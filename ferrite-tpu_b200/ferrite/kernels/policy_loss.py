@@ -46,8 +46,8 @@ def _launch(logits, targets, rest, clip, coefs, temperature, ignore_index, grad_
     rows, vocab = logits.shape
     old, adv, weights, ref = rest
     dev = logits.device
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    f = torch.empty((4, rows), dtype=torch.float32, device=dev)  # logp, entropy, kl, and the terms of the sum
+    loss = old.new_empty(())
+    f = old.new_empty((4, rows))  # logp, entropy, kl, and the terms of the sum
     base = f.data_ptr()
     clipped = torch.empty(rows, dtype=torch.bool, device=dev)
     grad = None if grad_dtype is None else _rows.empty_grad(logits, grad_dtype)

@@ -60,11 +60,11 @@ def _launch(logits, targets, ref, offsets, beta, kind, label_smoothing, average,
     rows, vocab = logits.shape
     pairs, dev = offsets.numel() // 2, logits.device
     keep = keep or grad_dtype is not None
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    per_pair = torch.empty((2, pairs), dtype=torch.float32, device=dev)  # margins and the terms of the mean
-    logp = torch.empty(rows, dtype=torch.float32, device=dev)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if keep else None
-    coef = torch.empty(rows, dtype=torch.float32, device=dev) if keep else None
+    loss = ref.new_empty(())
+    per_pair = ref.new_empty((2, pairs))  # margins and the terms of the mean
+    logp = ref.new_empty(rows)
+    stats = ref.new_empty((rows, 2)) if keep else None
+    coef = ref.new_empty(rows) if keep else None
     grad = None if grad_dtype is None else _rows.empty_grad(logits, grad_dtype)
     base = per_pair.data_ptr()
     nat.check(
