@@ -213,7 +213,7 @@ using namespace ferrite::rowloss;
 
 extern "C" {
 
-int ferrite_distill_loss(void* stream, const void* logits, const void* values, const void* indices, const float* weights, float temperature,
+int ferrite_distill_loss(void* stream, const void* logits, const void* values, const void* indices, const float* weights, double temperature,
                          const float* dloss, float scale, float* loss, float* per_token, void* dlogits, float* workspace,
                          size_t workspace_bytes, int64_t rows, int64_t vocab, int64_t top, int64_t ld, int64_t ld_out, int64_t ld_list,
                          int dtype, int value_dtype, int index_dtype, int out_dtype) {
@@ -234,7 +234,7 @@ int ferrite_distill_loss(void* stream, const void* logits, const void* values, c
       return fail(FERRITE_BAD_ALIGNMENT, "%s: misaligned pointer", op);
     const RowIn in = row_in(logits, rows, vocab, ld, temperature);
     const RowOut out{dlogits, ld_out, dloss, scale};
-    const Distill d{values, indices, ld_list, (int)top, value_dtype, index_dtype, weights, 1.f / (float)rows, temperature, workspace, per_token};
+    const Distill d{values, indices, ld_list, (int)top, value_dtype, index_dtype, weights, 1.f / (float)rows, (float)temperature, workspace, per_token};
     if (int rc = dispatch_row(s, in, out, d, dtype, dlogits ? out_dtype : -1, op)) return rc;
   }
   return sum_terms(s, workspace, loss, rows, 1.f, op);

@@ -306,7 +306,7 @@ using namespace ferrite::rowloss;
 extern "C" {
 
 int ferrite_logprobs_fwd(void* stream, const void* logits, const void* targets, float* logp, float* entropy, float* stats, int64_t rows,
-                         int64_t vocab, int64_t ld, int64_t ignore_index, float temperature, int dtype, int target_dtype) {
+                         int64_t vocab, int64_t ld, int64_t ignore_index, double temperature, int dtype, int target_dtype) {
   const char* op = "logprobs_fwd";
   if (int rc = check_rows(op, rows, vocab, ld, temperature, dtype, 0, -1)) return rc;
   if (int rc = check_targets(op, target_dtype)) return rc;
@@ -322,7 +322,7 @@ int ferrite_logprobs_fwd(void* stream, const void* logits, const void* targets, 
 
 int ferrite_logprobs_bwd(void* stream, const void* logits, const void* targets, const float* stats, const float* entropy,
                          const float* dlogp, const float* dentropy, const float* dloss, float scale, void* dlogits, int64_t rows,
-                         int64_t vocab, int64_t ld, int64_t ld_out, int64_t ignore_index, float temperature, int dtype, int target_dtype,
+                         int64_t vocab, int64_t ld, int64_t ld_out, int64_t ignore_index, double temperature, int dtype, int target_dtype,
                          int out_dtype) {
   const char* op = "logprobs_bwd";
   if (int rc = check_rows(op, rows, vocab, ld, temperature, dtype, ld_out, out_dtype < 0 ? 99 : out_dtype)) return rc;
@@ -341,7 +341,7 @@ int ferrite_logprobs_bwd(void* stream, const void* logits, const void* targets, 
 
 int ferrite_policy_loss(void* stream, const void* logits, const void* targets, const float* old_logp, const float* advantages,
                         const float* weights, const float* ref_logp, float clip_low, float clip_high, float kl_coef, float entropy_coef,
-                        float temperature, const float* dloss, float scale, float* loss, float* logp, float* entropy, float* kl,
+                        double temperature, const float* dloss, float scale, float* loss, float* logp, float* entropy, float* kl,
                         uint8_t* clipped, void* dlogits, float* workspace, size_t workspace_bytes, int64_t rows, int64_t vocab, int64_t ld,
                         int64_t ld_out, int64_t ignore_index, int dtype, int target_dtype, int out_dtype) {
   const char* op = "policy_loss";
@@ -387,7 +387,7 @@ int ferrite_preference_pairs(void* stream, const float* logp, const float* ref_l
 }
 
 int ferrite_preference_loss(void* stream, const void* logits, const void* targets, const float* ref_logp, const int64_t* offsets, float beta,
-                            float label_smoothing, int kind, int average, float temperature, float scale, float* loss, float* margins,
+                            float label_smoothing, int kind, int average, double temperature, float scale, float* loss, float* margins,
                             float* logp, float* stats, float* coef, void* dlogits, float* workspace, size_t workspace_bytes, int64_t rows,
                             int64_t pairs, int64_t vocab, int64_t ld, int64_t ld_out, int64_t ignore_index, int dtype, int target_dtype,
                             int out_dtype) {

@@ -197,13 +197,15 @@ __device__ __forceinline__ float y_of(float x, const Norm& w, const RowIn& in) {
   return w.big ? (x - w.base) * in.k : fmaf(x, in.k_lo, fmaf(x, in.k, -w.base));
 }
 // log p of one logit, rounded once: sums of it over long sequences show roundings that go one way, so
-// the difference is taken in f64, and s is relieved of what sums of ex2.approx are low by on average (7e-8:
-// between 4.5e-8 and 8.6e-8 measured over 2048 rows of 32000 against f64).
-constexpr double kEx2Low = 7e-8;
+// the difference is taken in f64.  ex2.approx is low by 6e-8 on average (between 3e-8 at 256 and 1.1e-7 at
+// 131072 columns, measured against f64 over 2000 to 60000 rows each), and so is the part of s that
+// is not the base's own term; to first order that moves log p up by the same times 1 - p.
+constexpr double kEx2Low = 6e-8;
 __device__ __forceinline__ float logp_of(float xt, const Norm& w, const RowIn& in) {
   const double k = (double)in.k + (double)in.k_lo;
   const double y = w.big ? (double)(xt - w.base) * k : (double)xt * k - (double)w.base;
-  return (float)((y - (double)log2f(w.s)) * 0.6931471805599453 - kEx2Low);
+  const double l = (y - (double)log2f(w.s)) * 0.6931471805599453;
+  return (float)(l - kEx2Low * (double)(1.f - ex2_approx((float)(y - (double)log2f(w.s)))));
 }
 __device__ __forceinline__ float entropy_of(const Norm& w) { return (log2f(w.s) - w.u / w.s) * kLn2; }
 
@@ -316,20 +318,20 @@ __device__ __forceinline__ Coef coef_of(float a, float b, float g, int64_t t, fl
 // --------------------------------------------------------------------------
 inline int elem_bytes(int dtype) { return dtype == FERRITE_F32 ? 4 : 2; }
 
-inline RowIn row_in(const void* logits, int64_t rows, int64_t vocab, int64_t ld, float temperature) {
-  const double k = 1.4426950408889634 / (double)temperature;
-  return RowIn{logits, rows, vocab, ld, (float)k, (float)(k - (double)(float)k), (float)(1.0 / (double)temperature)};
+inline RowIn row_in(const void* logits, int64_t rows, int64_t vocab, int64_t ld, double temperature) {
+  const double k = 1.4426950408889634 / temperature;
+  return RowIn{logits, rows, vocab, ld, (float)k, (float)(k - (double)(float)k), (float)(1.0 / temperature)};
 }
 
 // Sizes and types every entry point takes; `out_dtype` < 0 where there is no gradient.
-inline int check_rows(const char* op, int64_t rows, int64_t vocab, int64_t ld, float temperature, int dtype,
+inline int check_rows(const char* op, int64_t rows, int64_t vocab, int64_t ld, double temperature, int dtype,
                       int64_t ld_out, int out_dtype) {
   if (int rc = injected_fault(op)) return rc;
   if (rows < 0 || vocab <= 0 || ld < vocab)
     return fail(FERRITE_BAD_SHAPE, "%s: bad shape rows=%lld vocab=%lld ld=%lld", op, (long long)rows, (long long)vocab, (long long)ld);
   if (rows > 0x7fffffff || vocab > 0x7fffffff) return fail(FERRITE_BAD_SHAPE, "%s: more than 2^31 - 1 rows or columns", op);
-  if (!(temperature > 0.f) || !std::isfinite(temperature) || !std::isfinite(kLog2e / temperature))
-    return fail(FERRITE_BAD_SHAPE, "%s: temperature %g (it must be positive)", op, (double)temperature);
+  if (!(temperature > 0.0) || !std::isfinite((float)temperature) || !std::isfinite((float)(1.4426950408889634 / temperature)))
+    return fail(FERRITE_BAD_SHAPE, "%s: temperature %g (it must be positive)", op, temperature);
   if (dtype != FERRITE_F32 && dtype != FERRITE_BF16 && dtype != FERRITE_F16)
     return fail(FERRITE_UNSUPPORTED_DTYPE, "%s: logits dtype %d", op, dtype);
   if (out_dtype >= 0) {

@@ -50,6 +50,7 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _sz = ctypes.c_size_t
 
 
@@ -98,14 +99,14 @@ SIGNATURES: dict[str, tuple] = {
     "ferrite_adamw_step": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _f32, _f32, _f32, _f32, _f32, _i64, _f32, _f32, _vp, _vp, _sz]),
     "ferrite_xent_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32]),
     "ferrite_xent_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _f32, _vp, _i64, _i64, _i64, _i64, _i32, _i32]),
-    "ferrite_logprobs_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _i32, _i32]),
-    "ferrite_logprobs_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _i32]),
-    "ferrite_policy_loss": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _f32, _f32, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+    "ferrite_logprobs_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _f64, _i32, _i32]),
+    "ferrite_logprobs_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _vp, _i64, _i64, _i64, _i64, _i64, _f64, _i32, _i32, _i32]),
+    "ferrite_policy_loss": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _f32, _f32, _f32, _f32, _f64, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                    _sz, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32]),
     "ferrite_preference_pairs": (_i32, [_vp, _vp, _vp, _vp, _vp, _f32, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i32]),
-    "ferrite_preference_loss": (_i32, [_vp, _vp, _vp, _vp, _vp, _f32, _f32, _i32, _i32, _f32, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64,
+    "ferrite_preference_loss": (_i32, [_vp, _vp, _vp, _vp, _vp, _f32, _f32, _i32, _i32, _f64, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64,
                                        _i64, _i64, _i64, _i64, _i32, _i32, _i32]),
-    "ferrite_distill_loss": (_i32, [_vp, _vp, _vp, _vp, _vp, _f32, _vp, _f32, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
+    "ferrite_distill_loss": (_i32, [_vp, _vp, _vp, _vp, _vp, _f64, _vp, _f32, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
                                     _i32, _i32, _i32]),
     "ferrite_attn_bwd_ds_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i32]),
     "ferrite_attn_bwd_ds": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sp, _vp, _sz, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _i32, _i32]),

@@ -268,6 +268,9 @@ FERRITE_API int ferrite_xent_bwd(void* stream, const float* logits, const void* 
  *   - dlogits [rows, vocab] of `out_dtype` (dtype itself, or bf16 / f16 for f32 logits)
  *     with row stride ld_out; it must not overlap logits.  The gradient is that of the loss
  *     times (*dloss) * scale (dloss a device scalar, NULL meaning 1).
+ *   - a row's results do not depend on the call's other rows: the same logits, target and
+ *     temperature give the same bits in any batch, with a gradient or without, wherever the
+ *     row starts on a 16-byte boundary.
  *   - statistics, sums and losses are f32 (sums over rows are accumulated in f64, in a
  *     fixed order: results do not change from run to run).
  *   - a logit of -inf has p = 0 exactly; NaN or +inf makes the row's results NaN. */
@@ -276,14 +279,14 @@ FERRITE_API int ferrite_xent_bwd(void* stream, const float* logits, const void* 
  * a row for the backward. */
 FERRITE_API int ferrite_logprobs_fwd(void* stream, const void* logits, const void* targets, float* logp,
                         float* entropy, float* stats, int64_t rows, int64_t vocab, int64_t ld,
-                        int64_t ignore_index, float temperature, int dtype, int target_dtype);
+                        int64_t ignore_index, double temperature, int dtype, int target_dtype);
 
 /* dlogits of sum_r dlogp_r logp_r + dentropy_r H_r (either may be NULL: zero), from the
  * forward's stats and, with dentropy, its entropy. */
 FERRITE_API int ferrite_logprobs_bwd(void* stream, const void* logits, const void* targets, const float* stats,
                         const float* entropy, const float* dlogp, const float* dentropy,
                         const float* dloss, float scale, void* dlogits, int64_t rows, int64_t vocab,
-                        int64_t ld, int64_t ld_out, int64_t ignore_index, float temperature,
+                        int64_t ld, int64_t ld_out, int64_t ignore_index, double temperature,
                         int dtype, int target_dtype, int out_dtype);
 
 /* The clipped policy loss, and in the same pass its gradient when dlogits is given:
@@ -296,7 +299,7 @@ FERRITE_API int ferrite_logprobs_bwd(void* stream, const void* logits, const voi
 FERRITE_API int ferrite_policy_loss(void* stream, const void* logits, const void* targets, const float* old_logp,
                         const float* advantages, const float* weights, const float* ref_logp,
                         float clip_low, float clip_high, float kl_coef, float entropy_coef,
-                        float temperature, const float* dloss, float scale, float* loss, float* logp,
+                        double temperature, const float* dloss, float scale, float* loss, float* logp,
                         float* entropy, float* kl, uint8_t* clipped, void* dlogits, float* workspace,
                         size_t workspace_bytes, int64_t rows, int64_t vocab, int64_t ld, int64_t ld_out,
                         int64_t ignore_index, int dtype, int target_dtype, int out_dtype);
@@ -322,7 +325,7 @@ FERRITE_API int ferrite_preference_pairs(void* stream, const float* logp, const 
  * floats; stats: 2 rows floats (8-byte aligned); coef and stats may be NULL without dlogits. */
 FERRITE_API int ferrite_preference_loss(void* stream, const void* logits, const void* targets,
                         const float* ref_logp, const int64_t* offsets, float beta,
-                        float label_smoothing, int kind, int average, float temperature, float scale,
+                        float label_smoothing, int kind, int average, double temperature, float scale,
                         float* loss, float* margins, float* logp, float* stats, float* coef,
                         void* dlogits, float* workspace, size_t workspace_bytes, int64_t rows,
                         int64_t pairs, int64_t vocab, int64_t ld, int64_t ld_out,
@@ -337,7 +340,7 @@ FERRITE_API int ferrite_preference_loss(void* stream, const void* logits, const 
  * weight 0, is masked.  An index >= vocab gives NaN for the row.  A token listed twice
  * counts with both weights.  weights [rows] (NULL: 1 / rows).  workspace: rows floats. */
 FERRITE_API int ferrite_distill_loss(void* stream, const void* logits, const void* values, const void* indices,
-                        const float* weights, float temperature, const float* dloss, float scale,
+                        const float* weights, double temperature, const float* dloss, float scale,
                         float* loss, float* per_token, void* dlogits, float* workspace,
                         size_t workspace_bytes, int64_t rows, int64_t vocab, int64_t top, int64_t ld,
                         int64_t ld_out, int64_t ld_list, int dtype, int value_dtype, int index_dtype,
