@@ -608,6 +608,41 @@ def test_many_rows(rows, vocab, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,top", [(700, 100, 1024), (700, 3, 1000), (650, 20000, 1024), (900, 1, 1024), (640, 9000, 700)])
+def test_long_lists(rows, vocab, top):
+    """The longest lists, over vocabularies much smaller than they are (every token listed many times) and larger."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = 3 * torch.randn(rows, vocab, device="cuda", generator=g)
+    v, idx = torch.randn(rows, top, device="cuda", generator=g), torch.randint(-1, vocab, (rows, top), device="cuda", generator=g)
+    idx[5] = -1
+    ref = x.clone().requires_grad_(True)
+    want = distillation_loss_reference(ref, v, idx)
+    (gr,) = torch.autograd.grad(want.loss, ref)
+    got, gg = distillation_loss_and_grad(x, v, idx)
+    e = 4 * (tol(vocab) + tol(64 * top) + (vocab + top) * U) * (1 + np.log(vocab + 1) + np.log(top))
+    close(got.per_token, want.per_token.cpu().numpy().astype(np.float64), e)
+    close(gg, gr.cpu().numpy().astype(np.float64), e / rows * 2)
+    assert not gg[5].any() and got.per_token[5] == 0
+    nat.device_status()
+
+
+@pytest.mark.gpu
+def test_a_row_has_the_same_bits_in_every_batch():
+    """With 16-byte aligned rows a row's results and gradient depend on nothing but the row."""
+    for vocab, dtype in ((4096, torch.bfloat16), (32000, torch.bfloat16), (50304, torch.float32)):
+        g = torch.Generator(device="cuda").manual_seed(vocab)
+        x = (3 * torch.randn(1200, vocab, device="cuda", generator=g)).to(dtype)
+        t = torch.randint(0, vocab, (1200,), device="cuda", generator=g)
+        f = torch.randn(1200, device="cuda", generator=g)
+        w = torch.full((1200,), 0.5, device="cuda")
+        whole, grad = policy_loss_and_grad(x, t, f - 9, f, w, ref_logprobs=f - 9, kl_coef=0.01)
+        for a, b in ((0, 1), (7, 8), (300, 317), (1000, 1200)):
+            part, pg = policy_loss_and_grad(x[a:b].clone(), t[a:b], f[a:b] - 9, f[a:b], w[a:b], ref_logprobs=f[a:b] - 9, kl_coef=0.01)
+            assert torch.equal(part.logprobs, whole.logprobs[a:b]) and torch.equal(pg, grad[a:b]) and torch.equal(part.kl, whole.kl[a:b])
+        assert torch.equal(token_logprobs(x[300:317].clone(), t[300:317]), whole.logprobs[300:317])
+
+
+@pytest.mark.gpu
 def test_no_rows():
     x = torch.empty(0, 100, device="cuda")
     t, f = torch.empty(0, dtype=torch.long, device="cuda"), torch.empty(0, device="cuda")
