@@ -203,22 +203,22 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
 // Rows of 16 KB and more: one read from HBM, one write.
 //
 // Bound: HBM.  Both passes over a row (the sums, then the gradient) stream it through shared memory,
-// the second one from L2, where the rows in flight stay (296 CTAs x 125 KB are 37 MB): the first
+// the second one from L2, where the rows in flight stay (296 CTAs x 125 KB, 592 x 62.5 KB are 37 MB): the first
 // pass's copies ask L2 to keep them (evict_last), the second's let them go (evict_first).
 // The next bounds are instruction issue and the ex2 unit (16 a clock and SM; two per element, or one
 // without a gradient).
 //
-// Persistent CTAs, two to an SM (one where two rows an SM would not stay in L2: 1000 x 131072 f32 takes
-// 206 us with one, 240 with two; 16-bit rows half as long 119 and 115), take rows blockIdx, blockIdx + gridDim, ...  In a CTA
-//   - kGroups warps, one for each group below, issue untiled bulk copies of 16 KB chunks into a ring
+// Persistent CTAs, two or four to an SM (the layouts below; one where two rows an SM would not stay in L2:
+// 1000 x 131072 f32 takes 206 us with one, 240 with two; 16-bit rows half as long 119 and 115), take rows blockIdx, blockIdx + gridDim, ...  In a CTA
+//   - kGroups warps, one for each group below, issue untiled bulk copies of chunks into a ring
 //     (mbarriers full / empty), as far ahead as the ring allows.  The ring is a multiple of kGroups
 //     chunks, so that each of its places has one copy warp and one group for good.  (One warp for all
 //     of them takes about 600 cycles a copy -- its waits and its issue, one after the other -- and
 //     held reads to 3.7 TB/s with 8 KB copies.)
 //   - kGroups groups of four warps (one to each of the SM's quarters) run the passes, each on chunks
-//     of its own in turn.  The second pass of rows up to 64 KB runs one row behind the first (lag), so
-//     that nothing waits for what lies between a row's two passes (8192 x 32000 bf16: 201 us, else 207);
-//     with longer rows the two of each CTA no longer stay in L2 together (f32: 324 us, else 272);
+//     of its own in turn.  The second pass of shorter rows runs one row behind the first (lag), so that
+//     nothing waits for what lies between a row's two passes (two CTAs, 8192 x 32000 bf16: 201 us, else
+//     207); with longer rows the two of each CTA no longer stay in L2 together (f32: 324 us, else 272);
 //   - that is the work of kHelpers warps, rows in turn: fetch what the row's loss needs besides the
 //     logits (ahead of time), merge the passes' states, hand back the gradient's coefficients, write
 //     the row's results, and at last the single entries of a list.
@@ -226,29 +226,51 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
 // no copy is issued, nobody waits, and the copies in flight are waited for before the CTA exits.
 // --------------------------------------------------------------------------
 
-constexpr int kGroups = 2;
-constexpr int kGroup = 128;                     // threads of a group
-constexpr int kPass = kGroups * kGroup;         // threads of the passes
-constexpr int kWarps = kPass / 32;
-constexpr int kHelpers = 2;
-constexpr int kRingThreads = kPass + kGroups * 32 + kHelpers * 32;
-constexpr int kChunk = 16384;                   // bytes
-constexpr int kChunkVec = kChunk / 16;
-constexpr int kVecPer = kChunkVec / kGroup;     // vectors a thread takes of a chunk
-constexpr int kMaxChunks = 6;
-static_assert(kMaxChunks % kGroups == 0 && kMaxChunks <= 32, "places of one group each; a bit for each place");
+// How the kernel is laid out: GROUPS of four warps for the passes, a copy warp for each, HELPERS, and
+// CTAS of these to an SM; chunks of CHUNK bytes, PLACES of them in the ring; LAG: rows up to so many
+// bytes run with the second pass one row behind the first.
+template <int GROUPS, int HELPERS, int CTAS, int CHUNK, int PLACES, int64_t LAG>
+struct Layout {
+  static constexpr int kGroups = GROUPS, kHelpers = HELPERS, kCtas = CTAS, kChunk = CHUNK, kPlaces = PLACES;
+  static constexpr int64_t kLag = LAG;
+  static constexpr int kGroup = 128;                        // threads of a group
+  static constexpr int kPass = GROUPS * kGroup;             // threads of the passes
+  static constexpr int kWarps = kPass / 32;
+  static constexpr int kThreads = kPass + 128;              // one more group of four: copies, helpers, spare
+  static constexpr int kChunkVec = CHUNK / 16;
+  static constexpr int kVecPer = kChunkVec / kGroup;        // vectors a thread takes of a chunk
+  // registers go where the passes need them: (GROUPS * 88 + kSpare) * 128 = the launch's
+  static constexpr int kSpare = GROUPS == 1 ? 40 : 64;
+  static constexpr int kSmem = (227 - CTAS) * 1024 / CTAS / 128 * 128;  // of each CTA, besides what the system keeps
+  static_assert(GROUPS + HELPERS <= 4 && PLACES % GROUPS == 0 && PLACES <= 32, "warps of the fourth; places of one group each, a bit for each");
+  static_assert((GROUPS * 88 + kSpare) * 128 <= 65536 / CTAS / kThreads / 8 * 8 * kThreads, "registers of the launch");
+};
+// 16-bit rows up to 128 KB, four CTAs of one group: what a row costs whatever its length is paid by four warps
+// instead of eight, and three other CTAs fill the gaps (policy 8192 x 32000 bf16: 189 us against 200 for the
+// other layout, 8192 x 16384 109 against 125; 1000 x 131072 127 against 115).  Lists take 8 KB chunks
+// (distill 8192 x 32000 bf16: 203 us against 217 with 16 KB; policy 197 against 189).
+template <bool LIST>
+using NarrowLayout = Layout<1, 1, 4, LIST ? 8192 : 16384, LIST ? 6 : 3, 33 * 1024>;
+// Longer rows, and f32 rows, which have half the work to the byte (policy 8192 x 32000 f32: 259 us against 292).
+using WideLayout = Layout<2, 2, 2, 16384, 6, 64 * 1024>;
+constexpr int64_t kNarrowRow = 128 * 1024;
 
+template <class L>
 struct RingShared {
-  uint64_t full[kMaxChunks], empty[kMaxChunks];
+  uint64_t full[L::kPlaces], empty[L::kPlaces];
   // of a helper's row: its base is there; the passes' states are; its coefficients are; its
   // gradient is written
-  uint64_t ready[kHelpers], states[kHelpers], done[kHelpers], written[kHelpers];
-  State warp_state[kHelpers][kWarps];
-  alignas(16) Coef coef[kHelpers];
-  float base[kHelpers];
+  uint64_t ready[L::kHelpers], states[L::kHelpers], done[L::kHelpers], written[L::kHelpers];
+  State warp_state[L::kHelpers][L::kWarps];
+  alignas(16) Coef coef[L::kHelpers];
+  float base[L::kHelpers];
   int abort;
 };
-constexpr int kRingHeader = (int)((sizeof(RingShared) + 127) / 128 * 128);
+
+template <class L>
+__host__ __device__ constexpr int ring_header() {
+  return (int)((sizeof(RingShared<L>) + 127) / 128 * 128);
+}
 
 // The bounded wait of common.cuh for warps that run ahead of the passes: it sleeps between tries.
 __device__ __forceinline__ bool wait_idle(uint64_t* bar, uint32_t parity, volatile int* abort, int where) {
@@ -274,7 +296,7 @@ __device__ __forceinline__ void bulk_load_hint(void* dst, const void* src, uint3
 }
 
 // A row's chunks, kept from row to row while the rows' addresses agree modulo 16.
-template <typename T>
+template <typename T, int CHUNK_VEC>
 struct Chunks {
   int n, phase;
   int head, tail, nv, chunks;
@@ -287,7 +309,7 @@ struct Chunks {
     head = cut.head;
     tail = cut.tail;
     nv = cut.nv;
-    chunks = (nv + kChunkVec - 1) / kChunkVec;
+    chunks = (nv + CHUNK_VEC - 1) / CHUNK_VEC;
   }
   // the column of the element outside the vectors that thread tid takes, or -1
   __device__ __forceinline__ int edge(int tid) const {
@@ -333,14 +355,15 @@ struct Place {
   }
 };
 
-template <class Op, typename TI, typename TO, bool GRAD>
-__global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut out, Op op, int ring_chunks, int lag) {
-  constexpr int N = 16 / sizeof(TI);
+template <class L, class Op, typename TI, typename TO, bool GRAD>
+__global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, RowOut out, Op op, int ring_chunks, int lag) {
+  constexpr int N = 16 / sizeof(TI), kGroups = L::kGroups, kHelpers = L::kHelpers, kChunk = L::kChunk, kChunkVec = L::kChunkVec;
+  constexpr int kGroup = L::kGroup, kPass = L::kPass, kWarps = L::kWarps, kVecPer = L::kVecPer;
   constexpr bool kSums = !Op::kHasStats;        // a first pass
   constexpr bool kFix = GRAD && Op::kList;
   extern __shared__ __align__(128) char smem[];
-  RingShared& sh = *reinterpret_cast<RingShared*>(smem);
-  char* ring = smem + kRingHeader;
+  RingShared<L>& sh = *reinterpret_cast<RingShared<L>*>(smem);
+  char* ring = smem + ring_header<L>();
   const int slot_bytes = (op.slot_bytes() + 15) & ~15;
   char* slots = ring + (size_t)ring_chunks * kChunk;
   volatile int* abort = &sh.abort;
@@ -368,10 +391,9 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
   pdl_wait();
 
   LiveRows<Op> rows{op, in.rows, step, Op::kHasStats};
-  Chunks<TI> row((int)in.vocab);
-  // registers go where the passes need them: 256 x 88 + 128 x 64 = 384 x 80 of the launch
+  Chunks<TI, kChunkVec> row((int)in.vocab);
   if (warp >= kWarps) {
-    setmaxnreg_dec<64>();
+    setmaxnreg_dec<L::kSpare>();
     if (warp < kWarps + kGroups) {  // ---- copies of one group's chunks
       const int group = warp - kWarps;
       const uint64_t keep = l2_policy_evict_last(), let_go = l2_policy_evict_first();
@@ -429,7 +451,7 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
             }
         }
       }
-    } else {  // ---- what lies between a row's two passes
+    } else if (warp < kWarps + kGroups + kHelpers) {  // ---- what lies between a row's two passes
       const int h = warp - kWarps - kGroups;
       const float g = GRAD ? (out.dloss ? *out.dloss : 1.f) * out.scale : 0.f;
       int turn = 0;
@@ -660,9 +682,24 @@ __global__ void __launch_bounds__(kRingThreads, 2) ring_kernel(RowIn in, RowOut 
 // host
 // --------------------------------------------------------------------------
 
-constexpr int64_t kLagRow = 65536;      // bytes: the second pass of rows up to this runs a row behind the first
 constexpr int64_t kPairRow = 320 * 1024;  // bytes: of longer rows an SM takes one at a time
-constexpr int kRingSmem = (227 - 2) * 1024 / 2 / 128 * 128;  // of each of two CTAs, besides what the system keeps
+
+template <class L, class Op, typename TI, typename TO, bool GRAD>
+static cudaError_t launch_ring(cudaStream_t s, const RowIn& in, const RowOut& out, const Op& op, int dev) {
+  auto kern = ring_kernel<L, Op, TI, TO, GRAD>;
+  static std::atomic<bool> ready[64];  // (set once a device; racing first calls do the same)
+  if (!ready[dev].load(std::memory_order_relaxed)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    if (e != cudaSuccess) return e;
+    ready[dev].store(true, std::memory_order_relaxed);
+  }
+  const int slots = 2 * L::kHelpers * ((op.slot_bytes() + 15) & ~15);
+  int places = (L::kSmem - ring_header<L>() - slots) / L::kChunk;
+  places = (places < L::kPlaces ? places : L::kPlaces) / L::kGroups * L::kGroups;
+  const size_t smem = (size_t)ring_header<L>() + (size_t)places * L::kChunk + slots;
+  const int64_t bytes = in.vocab * (int64_t)sizeof(TI), ctas = (int64_t)num_sms(dev) * (bytes <= kPairRow ? L::kCtas : 1);
+  return launch_pdl(kern, dim3((unsigned)(in.rows < ctas ? in.rows : ctas)), dim3(L::kThreads), smem, s, in, out, op, places, bytes <= L::kLag);
+}
 
 template <class Op, typename TI, typename TO, bool GRAD>
 static int launch_row(cudaStream_t s, const RowIn& in, const RowOut& out, const Op& op, const char* name) {
@@ -673,24 +710,19 @@ static int launch_row(cudaStream_t s, const RowIn& in, const RowOut& out, const 
   // The kernel goes by the row's length and type (and a list's), not by how many rows there are, with a
   // gradient or without: so a row's results have the same bits in every call (log-probabilities taken
   // in one batch and compared in another differ by nothing), as long as it starts on a 16-byte boundary.
-  if (in.vocab * (int64_t)sizeof(TI) < kShortRow && kShortWarps * slot <= kShortSlots) {
+  const int64_t bytes = in.vocab * (int64_t)sizeof(TI);
+  if (bytes < kShortRow && kShortWarps * slot <= kShortSlots) {
     const int64_t ctas = (in.rows + kShortWarps - 1) / kShortWarps, most = (int64_t)num_sms(dev) * 16;
     e = launch_pdl(short_row_kernel<Op, TI, TO, GRAD>, dim3((unsigned)(ctas < most ? ctas : most)), dim3(kShortWarps * 32), kShortWarps * slot, s,
                    in, out, op);
   } else {
-    auto kern = ring_kernel<Op, TI, TO, GRAD>;
-    static std::atomic<bool> ready[64];  // (set once a device; racing first calls do the same)
-    if (!ready[dev].load(std::memory_order_relaxed)) {
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem);
-      if (e != cudaSuccess) return fail(FERRITE_LAUNCH_FAILED, "%s: shared memory attribute: %s", name, cudaGetErrorString(e));
-      ready[dev].store(true, std::memory_order_relaxed);
+    e = cudaSuccess;
+    bool narrow = false;
+    if constexpr (sizeof(TI) == 2) {
+      narrow = bytes <= kNarrowRow;
+      if (narrow) e = launch_ring<NarrowLayout<Op::kList>, Op, TI, TO, GRAD>(s, in, out, op, dev);
     }
-    int chunks = (kRingSmem - kRingHeader - 2 * kHelpers * slot) / kChunk;
-    chunks = (chunks < kMaxChunks ? chunks : kMaxChunks) / kGroups * kGroups;
-    const size_t smem = (size_t)kRingHeader + (size_t)chunks * kChunk + 2 * kHelpers * slot;
-    const int64_t ctas = (int64_t)num_sms(dev) * (in.vocab * (int64_t)sizeof(TI) <= kPairRow ? 2 : 1);
-    e = launch_pdl(kern, dim3((unsigned)(in.rows < ctas ? in.rows : ctas)), dim3(kRingThreads), smem, s, in, out, op, chunks,
-                   in.vocab * (int64_t)sizeof(TI) <= kLagRow);
+    if (!narrow) e = launch_ring<WideLayout, Op, TI, TO, GRAD>(s, in, out, op, dev);
   }
   if (e != cudaSuccess) return fail(FERRITE_LAUNCH_FAILED, "%s: %s", name, cudaGetErrorString(e));
   return check_launch(name);
