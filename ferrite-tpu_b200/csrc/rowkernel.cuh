@@ -239,11 +239,11 @@ struct Layout {
   static constexpr int kThreads = kPass + 128;              // one more group of four: copies, helpers, spare
   static constexpr int kChunkVec = CHUNK / 16;
   static constexpr int kVecPer = kChunkVec / kGroup;        // vectors a thread takes of a chunk
-  // registers go where the passes need them: (GROUPS * 88 + kSpare) * 128 = the launch's
-  static constexpr int kSpare = GROUPS == 1 ? 40 : 64;
+  // registers go where the passes need them: (GROUPS * kRegs + kSpareRegs) * 128, the launch's
+  static constexpr int kRegs = GROUPS == 1 ? 80 : 88, kSpareRegs = GROUPS == 1 ? 48 : 64;
   static constexpr int kSmem = (227 - CTAS) * 1024 / CTAS / 128 * 128;  // of each CTA, besides what the system keeps
   static_assert(GROUPS + HELPERS <= 4 && PLACES % GROUPS == 0 && PLACES <= 32, "warps of the fourth; places of one group each, a bit for each");
-  static_assert((GROUPS * 88 + kSpare) * 128 <= 65536 / CTAS / kThreads / 8 * 8 * kThreads, "registers of the launch");
+  static_assert((GROUPS * kRegs + kSpareRegs) * 128 <= 65536 / CTAS / kThreads / 8 * 8 * kThreads, "registers of the launch");
 };
 // 16-bit rows up to 128 KB, four CTAs of one group: what a row costs whatever its length is paid by four warps
 // instead of eight, and three other CTAs fill the gaps (policy 8192 x 32000 bf16: 189 us against 200 for the
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
   LiveRows<Op> rows{op, in.rows, step, Op::kHasStats};
   Chunks<TI, kChunkVec> row((int)in.vocab);
   if (warp >= kWarps) {
-    setmaxnreg_dec<L::kSpare>();
+    setmaxnreg_dec<L::kSpareRegs>();
     if (warp < kWarps + kGroups) {  // ---- copies of one group's chunks
       const int group = warp - kWarps;
       const uint64_t keep = l2_policy_evict_last(), let_go = l2_policy_evict_first();
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
       }
     }
   } else {  // ---- the passes
-    setmaxnreg_inc<88>();
+    setmaxnreg_inc<L::kRegs>();
     const Pairs2 kk(in);
     const uint32_t group = warp / (kGroup / 32), gtid = tid % kGroup;
     Place p, slot1, slot2;  // of the next pass's first chunk; of the helpers of the first and the second pass
@@ -605,8 +605,6 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
             uint4 raw[kVecPer];
 #pragma unroll
             for (int q = 0; q < kVecPer; ++q) raw[q] = v[q * kGroup];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.empty[at.at]);
 #pragma unroll
             for (int q = 0; q < kVecPer; ++q) {
               float vals[N], d[N];
@@ -630,9 +628,12 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
                 }
                 store_at(to + q * kGroup * N, d, vec);
               }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.empty[at.at]);
           }
+          // Released after the chunk's last use: its stores have what the loads brought, as in the first
+          // pass the check of the sums has.  Released right after the loads were issued, the next copy
+          // overtook some of them.
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[at.at]);
           at.next(ring_chunks, kGroups);
           left -= kGroups * kChunkVec;
           to += kGroups * kChunkVec * N;

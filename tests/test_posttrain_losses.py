@@ -643,6 +643,46 @@ def test_a_row_has_the_same_bits_in_every_batch():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,dtype", [(6000, 32000, "bf16"), (6000, 8192, "bf16"), (8000, 4096, "f16"), (3000, 32000, "f32"), (2500, 50264, "f16"), (1200, 131072, "bf16"), (500, 200000, "f32")])
+def test_full_gpu_repeats_and_matches_small_batches(rows, vocab, dtype):
+    """With every SM busy, calls back to back give the same bits each time, and those of a few rows alone: no
+    entry comes from a piece of a row that was overwritten while it was in use."""
+    g = torch.Generator(device="cuda").manual_seed(rows + vocab)
+    x = (3 * torch.randn(rows, vocab, device="cuda", generator=g)).to(TORCH[dtype])
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    f, dlp = torch.randn(2, rows, device="cuda", generator=g)
+    w = torch.full((rows,), 1.0 / rows, device="cuda")
+    v, idx = torch.randn(rows, 4096, device="cuda", generator=g).topk(64)
+    off = torch.arange(0, rows + 1, rows // 10, device="cuda")
+
+    def logprobs(a, b):
+        leaf = x[a:b].detach().requires_grad_(True)
+        lp, h = token_logprobs(leaf, t[a:b], entropy=True)
+        (grad,) = torch.autograd.grad([lp, h], [leaf], [dlp[a:b], 0.1 * dlp[a:b]])
+        return lp.detach(), h.detach(), grad
+
+    def policy(a, b):
+        out, grad = policy_loss_and_grad(x[a:b], t[a:b], f[a:b] - 9, dlp[a:b], w[a:b], ref_logprobs=f[a:b] - 9, kl_coef=0.01)
+        return out.logprobs, out.kl, grad
+
+    def distill(a, b):
+        out, grad = distillation_loss_and_grad(x[a:b], v[a:b], idx[a:b], w[a:b])
+        return out.per_token, grad
+
+    for fn in (logprobs, policy, distill):
+        first = fn(0, rows)
+        for _ in range(6):
+            assert all(torch.equal(p, q) for p, q in zip(fn(0, rows), first))
+        for a in range(0, rows, rows // 5):
+            part = fn(a, a + 60)
+            assert all(torch.equal(p, q[a:a + 60]) for p, q in zip(part, first))
+    out, first = preference_loss_and_grad(x, t, f - 9, off)
+    for _ in range(6):
+        again, grad = preference_loss_and_grad(x, t, f - 9, off)
+        assert torch.equal(grad, first) and torch.equal(again.loss, out.loss)
+
+
+@pytest.mark.gpu
 def test_no_rows():
     x = torch.empty(0, 100, device="cuda")
     t, f = torch.empty(0, dtype=torch.long, device="cuda"), torch.empty(0, device="cuda")
