@@ -15,8 +15,11 @@
 // on store.
 //
 // y_i is K x_i - c with c = k m rounded -- one number for every term of s and for logp, so that its
-// rounding cancels -- and K = k + k_lo carried to twice f32: the rounding of k alone would shift
-// every log-probability the same way, and sums over long sequences would show it.  Where |c| passes
+// rounding cancels -- and K is carried to more than f32: the rounding of k alone would shift every
+// log-probability the same way, and sums over long sequences would show it.  The sums take K as
+// k_hi + k_rest, two fma: split after 12 bits, because the rest of a split after 24 is less than half
+// a unit of a y of 4 or more and would be rounded away each time; positive, because -inf times a rest
+// of 0 or below would be NaN.  Where |c| passes
 // 2^16 (logits in the tens of thousands, rows of the type's lowest value, infinities) y_i is
 // k (x_i - m) with m the maximum.  At its end a row is normalised: c takes up log2 s, so that s is
 // 1 but for rounding and log p = ln2 y loses nothing to cancellation.  A logit of -inf has e_i = 0
@@ -46,7 +49,8 @@ __device__ __forceinline__ State empty_state(float base = -INFINITY) { return St
 struct RowIn {
   const void* logits;
   int64_t rows, vocab, ld;
-  float k, k_lo;  // log2(e) / tau, and what its rounding left
+  float k, k_lo;      // log2(e) / tau, and what its rounding left
+  float k_hi, k_rest;  // the same split after 12 bits, k_rest > 0
   float inv_tau;  // 1 / tau
 };
 struct RowOut {
@@ -120,7 +124,7 @@ __device__ __forceinline__ void push_any(State& st, const float (&x)[N], const R
     if (st.m == -INFINITY) {  // nothing but -inf so far
       if (x[i] != x[i]) st.s = x[i];
     } else {
-      const float y = is_big(c) ? (x[i] - st.m) * in.k : fmaf(x[i], in.k_lo, fmaf(x[i], in.k, -c));
+      const float y = is_big(c) ? (x[i] - st.m) * in.k : fmaf(x[i], in.k_rest, fmaf(x[i], in.k_hi, -c));
       const float e = ex2_approx(y);
       st.s += e;
       if constexpr (ENT) st.u += e > 0.f ? e * y : 0.f;
@@ -134,10 +138,10 @@ __device__ __forceinline__ float minus_c(float m, const RowIn& in) {
   return is_big(c) ? __int_as_float(0x7fc00000) : -c;
 }
 
-// k and k_lo in both halves of register pairs.
+// k, k_hi and k_rest in both halves of register pairs.
 struct Pairs2 {
-  uint64_t k, k_lo;
-  __device__ __forceinline__ explicit Pairs2(const RowIn& in) : k(f2_make(in.k, in.k)), k_lo(f2_make(in.k_lo, in.k_lo)) {}
+  uint64_t k, k_hi, k_rest;
+  __device__ __forceinline__ explicit Pairs2(const RowIn& in) : k(f2_make(in.k, in.k)), k_hi(f2_make(in.k_hi, in.k_hi)), k_rest(f2_make(in.k_rest, in.k_rest)) {}
 };
 
 // Sums of the usual values: per pair of elements two packed fma (y), two ex2 and packed adds.  They
@@ -148,7 +152,7 @@ __device__ __forceinline__ void sum_usual(uint64_t& s2, uint64_t& u2, const floa
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
     const uint64_t x2 = f2_make(x[i], x[i + 1]);
-    const uint64_t y2 = f2_fma(x2, kk.k_lo, f2_fma(x2, kk.k, c2));
+    const uint64_t y2 = f2_fma(x2, kk.k_rest, f2_fma(x2, kk.k_hi, c2));
     const uint64_t e2 = f2_make(ex2_approx(f2_lo(y2)), ex2_approx(f2_hi(y2)));
     s2 = f2_add(s2, e2);
     if constexpr (ENT) u2 = f2_fma(e2, y2, u2);  // -inf: 0 * -inf = NaN, and not usual
@@ -194,18 +198,19 @@ __device__ __forceinline__ Norm normalise(const State& st, const RowIn& in) {
   return Norm{c2, s, ENT ? s * (st.u / st.s - l + err) : 0.f, 0};
 }
 __device__ __forceinline__ float y_of(float x, const Norm& w, const RowIn& in) {
-  return w.big ? (x - w.base) * in.k : fmaf(x, in.k_lo, fmaf(x, in.k, -w.base));
+  return w.big ? (x - w.base) * in.k : fmaf(x, in.k_rest, fmaf(x, in.k_hi, -w.base));
 }
 // log p of one logit, rounded once: sums of it over long sequences show roundings that go one way, so
-// the difference is taken in f64.  ex2.approx is low by 6e-8 on average (between 3e-8 at 256 and 1.1e-7 at
-// 131072 columns, measured against f64 over 2000 to 60000 rows each), and so is the part of s that
-// is not the base's own term; to first order that moves log p up by the same times 1 - p.
-constexpr double kEx2Low = 6e-8;
+// the difference is taken in f64.  The mean error of ex2.approx, measured against f64 over 10^7 values an
+// octave, is -5.1e-8 below y = -1 and 3.4e-8 above y = 1; s has it in all but the base's own term, so to first
+// order log p moves by the opposite times 1 - p.  Which of the two: most of s lies below a target of more than
+// a few times the mean probability (log p then off by 3e-8 at most on average, from 256 to 131072 columns).
+constexpr float kEx2Below = -5.1e-8f, kEx2Above = 3.4e-8f, kEx2Turn = 4.f;
 __device__ __forceinline__ float logp_of(float xt, const Norm& w, const RowIn& in) {
   const double k = (double)in.k + (double)in.k_lo;
-  const double y = w.big ? (double)(xt - w.base) * k : (double)xt * k - (double)w.base;
-  const double l = (y - (double)log2f(w.s)) * 0.6931471805599453;
-  return (float)(l - kEx2Low * (double)(1.f - ex2_approx((float)(y - (double)log2f(w.s)))));
+  const double y = (w.big ? (double)(xt - w.base) * k : (double)xt * k - (double)w.base) - (double)log2f(w.s);
+  const float p = ex2_approx((float)y);
+  return (float)(y * 0.6931471805599453 + (double)((p * (float)in.vocab > kEx2Turn ? kEx2Below : kEx2Above) * (1.f - p)));
 }
 __device__ __forceinline__ float entropy_of(const Norm& w) { return (log2f(w.s) - w.u / w.s) * kLn2; }
 
@@ -320,7 +325,10 @@ inline int elem_bytes(int dtype) { return dtype == FERRITE_F32 ? 4 : 2; }
 
 inline RowIn row_in(const void* logits, int64_t rows, int64_t vocab, int64_t ld, double temperature) {
   const double k = 1.4426950408889634 / temperature;
-  return RowIn{logits, rows, vocab, ld, (float)k, (float)(k - (double)(float)k), (float)(1.0 / temperature)};
+  int e = 0;
+  const double f = std::frexp(k, &e);
+  const float k_hi = (float)std::ldexp(std::floor(f * 4096.0) - 1.0, e - 12);  // below k: k_rest > 0
+  return RowIn{logits, rows, vocab, ld, (float)k, (float)(k - (double)(float)k), k_hi, (float)(k - (double)k_hi), (float)(1.0 / temperature)};
 }
 
 // Sizes and types every entry point takes; `out_dtype` < 0 where there is no gradient.

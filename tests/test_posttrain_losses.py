@@ -493,6 +493,34 @@ def test_masked_vocabulary(dtype, low):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("vocab", [1500, 32000])
+@pytest.mark.parametrize("tau", [0.7, 0.8, 1.0, 1.4426950408889634, 3.0])
+def test_masked_vocabulary_at_any_temperature(dtype, vocab, tau):
+    """-inf columns, whatever sign the rounding error of log2(e) / tau has (0 for tau = log2 e)."""
+    rng = np.random.default_rng(40)
+    x = logits_of(rng, 4, vocab, dtype)
+    hide = rng.random(vocab) < 0.4
+    hide[:300] = True
+    x[:, hide] = -np.inf
+    keep = np.flatnonzero(~hide)
+    t = rng.choice(keep, 4)
+    want, wh = op.token_logprobs(x[:, ~hide], np.searchsorted(keep, t), tau)
+    xt, tt = to_torch(x).requires_grad_(True), torch.from_numpy(t).cuda()
+    lp = token_logprobs(xt, tt, temperature=tau)
+    close(lp, want, tol(vocab) * (1 + np.abs(want)))
+    both, h = token_logprobs(xt, tt, entropy=True, temperature=tau)
+    close(both, want, tol(vocab) * (1 + np.abs(want)))
+    close(h, wh, 2 * tol(vocab) * (2 + wh + 8))
+    f = torch.ones(4, device="cuda")
+    out, g = policy_loss_and_grad(xt.detach(), tt, lp.detach(), f, f, temperature=tau)
+    assert torch.isfinite(out.loss) and torch.isfinite(g).all() and not g[:, torch.from_numpy(hide).cuda()].any()
+    idx = torch.from_numpy(np.stack([rng.choice(keep, 20, replace=False) for _ in range(4)])).cuda()
+    out, g = distillation_loss_and_grad(xt.detach(), torch.randn(4, 20, device="cuda"), idx, temperature=tau)
+    assert torch.isfinite(out.per_token).all() and torch.isfinite(g).all() and not g[:, torch.from_numpy(hide).cuda()].any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_rows_of_one_value(dtype):
     """Rows whose every logit is the same -- zero, a large value, the type's lowest or highest -- are uniform."""
