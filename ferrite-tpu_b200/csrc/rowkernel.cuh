@@ -79,8 +79,9 @@ __device__ __forceinline__ bool push_usual(State& st, float nc, const uint4 (&ra
 // --------------------------------------------------------------------------
 // Short rows: a warp per row, which reads it twice (the second time from L1 or L2).  No barriers; many
 // rows in flight hide the latency of each.  Bound by that latency and by the work of a row that does
-// not grow with it.  At 16 KB the other kernel's stream of copies wins (policy, 16384 x 8192 bf16: 171 us
-// against 195; half as long rows 158 against 89).
+// not grow with it.  From 16 KB on the two are close (policy, 16384 x 8192 bf16: 132 us
+// against the other kernel's 136) and the other's copies keep up with longer rows; half as long rows take 68 us
+// against its 126.
 // --------------------------------------------------------------------------
 
 constexpr int kShortWarps = 4;                 // rows of a CTA
@@ -248,7 +249,7 @@ struct Layout {
 // 16-bit rows up to 128 KB, four CTAs of one group: what a row costs whatever its length is paid by four warps
 // instead of eight, and three other CTAs fill the gaps (policy 8192 x 32000 bf16: 189 us against 200 for the
 // other layout, 8192 x 16384 109 against 125; 1000 x 131072 127 against 115).  Lists take 8 KB chunks
-// (distill 8192 x 32000 bf16: 203 us against 217 with 16 KB; policy 197 against 189).
+// (distill 8192 x 32000 bf16: 200 us against 207 with 16 KB; policy 197 against 189).
 template <bool LIST>
 using NarrowLayout = Layout<1, 1, 4, LIST ? 8192 : 16384, LIST ? 6 : 3, 33 * 1024>;
 // Longer rows, and f32 rows, which have half the work to the byte (policy 8192 x 32000 f32: 259 us against 292).
