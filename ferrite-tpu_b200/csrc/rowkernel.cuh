@@ -230,8 +230,16 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
 // How the kernel is laid out: GROUPS of four warps for the passes, a copy warp for each, HELPERS, and
 // CTAS of these to an SM; chunks of CHUNK bytes, PLACES of them in the ring; LAG: rows up to so many
 // bytes run with the second pass one row behind the first.
-template <int GROUPS, int HELPERS, int CTAS, int CHUNK, int PLACES, int64_t LAG>
+//
+// A helper has one place for its row's coefficients.  It writes row i's once every warp has handed in the states
+// of row i, so every warp must have read those of its row before by then, row i - HELPERS.  Without lag a warp
+// reads row i - 1's ahead of the states of row i.  With lag its order is first(i - 1), second(i - 2), first(i): it has
+// read those of row i - 2 and not yet those of row i - 1, so that two helpers are needed, or a helper that waits
+// until its row's gradient is written before it goes on to its next (lists).
+template <int GROUPS, int HELPERS, int CTAS, int CHUNK, int PLACES, int64_t LAG, bool WAITS>
 struct Layout {
+  static_assert(LAG == 0 || HELPERS >= 2 || WAITS, "the coefficients of a row behind would be overwritten");
+  static constexpr bool kWaits = WAITS;
   static constexpr int kGroups = GROUPS, kHelpers = HELPERS, kCtas = CTAS, kChunk = CHUNK, kPlaces = PLACES;
   static constexpr int64_t kLag = LAG;
   static constexpr int kGroup = 128;                        // threads of a group
@@ -251,9 +259,9 @@ struct Layout {
 // other layout, 8192 x 16384 109 against 125; 1000 x 131072 127 against 115).  Lists take 8 KB chunks
 // (distill 8192 x 32000 bf16: 200 us against 207 with 16 KB; policy 197 against 189).
 template <bool LIST>
-using NarrowLayout = Layout<1, 1, 4, LIST ? 8192 : 16384, LIST ? 6 : 3, 33 * 1024>;
+using NarrowLayout = Layout<1, LIST ? 1 : 2, 4, LIST ? 8192 : 16384, LIST ? 6 : 3, 33 * 1024, LIST>;
 // Longer rows, and f32 rows, which have half the work to the byte (policy 8192 x 32000 f32: 259 us against 292).
-using WideLayout = Layout<2, 2, 2, 16384, 6, 64 * 1024>;
+using WideLayout = Layout<2, 2, 2, 16384, 6, 64 * 1024, false>;
 constexpr int64_t kNarrowRow = 128 * 1024;
 
 template <class L>
@@ -362,6 +370,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
   constexpr int kGroup = L::kGroup, kPass = L::kPass, kWarps = L::kWarps, kVecPer = L::kVecPer;
   constexpr bool kSums = !Op::kHasStats;        // a first pass
   constexpr bool kFix = GRAD && Op::kList;
+  static_assert(!L::kWaits || Op::kList, "a layout that counts on its helpers' wait for the gradient");
   extern __shared__ __align__(128) char smem[];
   RingShared<L>& sh = *reinterpret_cast<RingShared<L>*>(smem);
   char* ring = smem + ring_header<L>();

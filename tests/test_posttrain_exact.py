@@ -1,0 +1,90 @@
+"""The post-training losses against their formulas in 64 bits, on the GPU, where a short test cannot reach:
+every entry of gradients that take the whole GPU, rows that start anywhere, unlikely targets, wide margins.
+
+Tolerances.  u = 2^-24 and ``tol(V) = (96 + V / 64) u`` bound the relative error of a row's sum, of a probability,
+and the absolute one of a log-probability's 2^y terms (an exponential off by 2^-22, the rounding of y by at most 64 u for
+|y| <= 128, V / 64 + 32 additions).  A coefficient a = dL/dlogp is off by its own formula's share of the
+log-probability's error; a stored gradient by half a step of its type besides.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from ferrite import _native as nat
+from ferrite.kernels.policy_loss import policy_loss_and_grad
+
+U = 2.0**-24
+IGN = -100
+TORCH = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def tol(vocab):
+    return (96 + vocab / 64) * U
+
+
+def stored(g, dtype):
+    """What storing g as ``dtype`` may change it by: half a step, and half of the smallest f16."""
+    step = {torch.float32: U, torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}[dtype]
+    return step * g.abs() + (2.0**-25 if dtype == torch.float16 else 1e-38)
+
+
+def softmax64(x, tau=1.0):
+    """(log p, p, H) of rows of logits, in 64 bits."""
+    lp = torch.log_softmax(x.double() / tau, 1)
+    p = lp.exp()
+    return lp, p, -torch.where(p > 0, p * lp, 0.0).sum(1)
+
+
+def check_policy_grad(grad, x, t, old, adv, w, ref, beta, c, lo=0.2, hi=0.2, tau=1.0):
+    """Every entry of the policy loss's gradient, slice by slice: w (a ([i = t] - p) + c p (log p + H)) / tau."""
+    vocab = x.shape[1]
+    for a in range(0, len(t), 500):
+        s = slice(a, a + 500)
+        lp, p, h = softmax64(x[s], tau)
+        logp = lp.gather(1, t[s, None])[:, 0]
+        ratio = (logp - old[s].double()).exp()
+        free, held = ratio * adv[s], ratio.clamp(1 - lo, 1 + hi) * adv[s]
+        d = ref[s].double() - logp
+        co = w[s].double() * (torch.where(held < free, 0.0, -free) - beta * torch.expm1(d))
+        one = torch.zeros_like(p)
+        one[torch.arange(len(logp), device=x.device), t[s]] = 1.0
+        own = c * w[s].double()
+        want = (co[:, None] * (one - p) + own[:, None] * p * (lp.clamp_min(-1e5) + h[:, None])) / tau
+        # the coefficient's error: that of logp, in exp(logp - old) and exp(ref - logp), and their roundings
+        e = tol(vocab) * (1 + logp.abs()) + 4 * U * (1 + old[s].abs() + ref[s].abs())
+        amp = co.abs() * tol(vocab) + w[s].double() * (free.abs() + beta * d.exp()) * e
+        bound = (amp[:, None] * (p + one) + 2 * tol(vocab) * (co.abs() + own)[:, None] * p * (1 + lp.abs().clamp_max(1e5) + h[:, None])) / tau
+        bad = (grad[s].double() - want).abs() > 2 * bound + 1.01 * stored(want, grad.dtype)
+        assert not bad.any(), f"{int(bad.sum())} entries off, the first in row {a + int(bad.any(1).nonzero()[0])}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,dtype", [(4000, 8203, "bf16"), (3500, 12345, "f16"), (3000, 16001, "bf16"), (3000, 8192, "f16"), (3000, 16384, "bf16")])
+@pytest.mark.parametrize("c", [0.0, 0.01])
+def test_rows_whose_gradient_runs_behind(rows, vocab, dtype, c):
+    """16-bit rows of 16 to 33 KB, several to a CTA, on and off 16-byte boundaries, some masked: every entry of the
+    policy gradient, the same bits in every call, and those of a few rows alone."""
+    g = torch.Generator(device="cuda").manual_seed(rows + vocab)
+    x = (3 * torch.randn(rows, vocab, device="cuda", generator=g)).to(TORCH[dtype])
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    # rows that differ in everything that reaches their coefficients
+    logp = torch.cat([torch.log_softmax(x[a : a + 500].float(), 1).gather(1, t[a : a + 500, None])[:, 0] for a in range(0, rows, 500)])
+    old, ref = logp + 0.1 * torch.randn(rows, device="cuda", generator=g), logp + 0.3 * torch.randn(rows, device="cuda", generator=g)
+    adv = torch.randn(rows, device="cuda", generator=g)
+    w = torch.rand(rows, device="cuda", generator=g) * (torch.rand(rows, device="cuda", generator=g) > 0.1)
+
+    def call(a, b):
+        out, grad = policy_loss_and_grad(x[a:b], t[a:b], old[a:b], adv[a:b], w[a:b], ref_logprobs=ref[a:b], kl_coef=0.05, entropy_coef=c)
+        return out.logprobs, out.entropy, out.kl, out.clipped, grad
+
+    first = call(0, rows)
+    edge = (torch.where(adv > 0, first[0] - old - np.log(1.2), first[0] - old - np.log(0.8))).abs() < 1e-4  # either side of a clipping bound
+    keep = ~edge
+    check_policy_grad(first[4][keep], x[keep], t[keep], old[keep], adv[keep], w[keep], ref[keep], 0.05, c)
+    for _ in range(20):
+        assert all(torch.equal(p, q) for p, q in zip(call(0, rows), first))
+    for a in range(0, rows, rows // 7):
+        b = min(rows, a + 50)
+        assert all(torch.equal(p, q[a:b]) for p, q in zip(call(a, b), first))
+    nat.device_status()
