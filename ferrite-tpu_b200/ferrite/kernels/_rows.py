@@ -86,7 +86,7 @@ def check_temperature(temperature: float) -> float:
 
 def upstream(g: torch.Tensor) -> torch.Tensor:
     """The gradient of a scalar loss as a dense f32 device scalar."""
-    return g.reshape(()).to(torch.float32).contiguous()
+    return g.detach().reshape(()).to(torch.float32).contiguous()
 
 
 def same_device(logits: torch.Tensor, *others: torch.Tensor | None) -> None:

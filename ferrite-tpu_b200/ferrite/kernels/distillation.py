@@ -96,12 +96,14 @@ def distillation_loss(logits, teacher_values, teacher_indices, weights=None, *, 
 
 @nat.on_tensor_device
 def distillation_loss_and_grad(logits, teacher_values, teacher_indices, weights=None, *, temperature: float = 1.0, grad_scale: float = 1.0,
-                               grad_dtype=None) -> tuple[DistillationLoss, torch.Tensor]:
+                               grad_dtype=None, upstream: torch.Tensor | None = None) -> tuple[DistillationLoss, torch.Tensor]:
     """:func:`distillation_loss` and ``grad_scale`` times its gradient in the logits, in one pass over
-    them; ``grad_dtype`` defaults to the logits' type (f32 logits also give bf16 or f16)."""
+    them; ``grad_dtype`` defaults to the logits' type (f32 logits also give bf16 or f16).  ``upstream``, a scalar
+    on the device, multiplies the gradient as well, before it is rounded."""
     grad_dtype = grad_dtype or logits.dtype
     values, indices, weights, temperature = _check(logits, teacher_values, teacher_indices, weights, temperature, grad_dtype)
-    return _launch(logits, values, indices, weights, temperature, grad_dtype, None, float(grad_scale))
+    dloss = None if upstream is None else _rows.upstream(upstream)
+    return _launch(logits, values, indices, weights, temperature, grad_dtype, dloss, float(grad_scale))
 
 
 def distillation_loss_reference(logits, teacher_values, teacher_indices, weights=None, *, temperature=1.0) -> DistillationLoss:

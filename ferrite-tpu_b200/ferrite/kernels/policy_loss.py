@@ -102,13 +102,16 @@ def policy_loss(logits, targets, old_logprobs, advantages, weights=None, *, ref_
 @nat.on_tensor_device
 def policy_loss_and_grad(logits, targets, old_logprobs, advantages, weights=None, *, ref_logprobs=None, clip_low: float = 0.2,
                          clip_high: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0, temperature: float = 1.0,
-                         ignore_index: int = IGNORE_INDEX, grad_scale: float = 1.0, grad_dtype=None) -> tuple[PolicyLoss, torch.Tensor]:
+                         ignore_index: int = IGNORE_INDEX, grad_scale: float = 1.0, grad_dtype=None,
+                         upstream: torch.Tensor | None = None) -> tuple[PolicyLoss, torch.Tensor]:
     """:func:`policy_loss` and ``grad_scale`` times its gradient in the logits, in one pass over
-    them; ``grad_dtype`` defaults to the logits' type (f32 logits also give bf16 or f16)."""
+    them; ``grad_dtype`` defaults to the logits' type (f32 logits also give bf16 or f16).  ``upstream``, a scalar
+    on the device, multiplies the gradient as well, before it is rounded."""
     grad_dtype = grad_dtype or logits.dtype
     targets, rest, temperature = _check(logits, targets, old_logprobs, advantages, weights, ref_logprobs, clip_low, clip_high, temperature, grad_dtype)
+    dloss = None if upstream is None else _rows.upstream(upstream)
     return _launch(logits, targets, rest, (float(clip_low), float(clip_high)), (float(kl_coef), float(entropy_coef)), temperature,
-                   int(ignore_index), grad_dtype, None, float(grad_scale))
+                   int(ignore_index), grad_dtype, dloss, float(grad_scale))
 
 
 def policy_loss_reference(logits, targets, old_logprobs, advantages, weights=None, *, ref_logprobs=None, clip_low=0.2, clip_high=0.2,

@@ -117,13 +117,16 @@ def preference_loss(logits, targets, ref_logprobs, offsets, *, beta: float = 0.1
 @nat.on_tensor_device
 def preference_loss_and_grad(logits, targets, ref_logprobs, offsets, *, beta: float = 0.1, kind: str = "sigmoid", label_smoothing: float = 0.0,
                              average: bool = False, temperature: float = 1.0, ignore_index: int = IGNORE_INDEX, grad_scale: float = 1.0,
-                             grad_dtype=None) -> tuple[PreferenceLoss, torch.Tensor]:
+                             grad_dtype=None, upstream: torch.Tensor | None = None) -> tuple[PreferenceLoss, torch.Tensor]:
     """:func:`preference_loss` and ``grad_scale`` times its gradient in the logits; ``grad_dtype``
-    defaults to the logits' type (f32 logits also give bf16 or f16)."""
+    defaults to the logits' type (f32 logits also give bf16 or f16).  ``upstream``, a scalar on the device, multiplies
+    the gradient as well, before it is rounded."""
     grad_dtype = grad_dtype or logits.dtype
     targets, ref, offsets, temperature = _check(logits, targets, ref_logprobs, offsets, beta, kind, label_smoothing, temperature, grad_dtype)
-    out, _, _, grad = _launch(logits, targets, ref, offsets, float(beta), kind, float(label_smoothing), average, temperature, int(ignore_index),
-                              True, grad_dtype, float(grad_scale))
+    out, stats, coef, grad = _launch(logits, targets, ref, offsets, float(beta), kind, float(label_smoothing), average, temperature, int(ignore_index),
+                                     True, grad_dtype if upstream is None else None, float(grad_scale))
+    if upstream is not None:
+        grad = logprobs_backward(logits, targets, stats, None, coef, None, _rows.upstream(upstream), float(grad_scale), temperature, int(ignore_index), grad_dtype)
     return out, grad
 
 
