@@ -68,6 +68,9 @@ def _products(ctx, dl, y, e):
 
 
 def _apply(y, e, loss, loss_and_grad, args, kw, logits_dtype):
+    for name in ("grad_scale", "grad_dtype", "upstream"):
+        if name in kw:
+            raise TypeError(f"{name} is of the logits' own gradient; the gradients of y and the embedding are autograd's")
     if y.ndim != 2 or e.ndim != 2 or y.shape[1] != e.shape[1]:
         raise ValueError(f"expected y [rows, d] and e [vocab, d]; got {tuple(y.shape)} and {tuple(e.shape)}")
     if y.dtype != e.dtype:

@@ -47,3 +47,15 @@ def test_f16_gradients_have_the_upstream_scale_before_they_are_rounded(which, lo
     for a, b in ((y.grad, y2.grad), (e.grad, e2.grad)):
         assert a.dtype == torch.float16
         assert (a.float() - b).abs().max().item() <= 2.0**-9 * b.abs().max().item()
+
+
+def test_scales_of_the_logits_gradient_are_refused():
+    """The node's gradient is autograd's: what scales or rounds the logits' own is not an argument of these."""
+    y, e, t, f = torch.zeros(4, 8), torch.zeros(16, 8), torch.zeros(4, dtype=torch.long), torch.zeros(4)
+    for kw in ({"grad_scale": 1024.0}, {"grad_dtype": torch.float32}):
+        with pytest.raises(TypeError, match=next(iter(kw))):
+            tied_head_policy_loss(y, e, t, f, f, **kw)
+        with pytest.raises(TypeError, match=next(iter(kw))):
+            tied_head_preference_loss(y, e, t, f, torch.tensor([0, 2, 4]), **kw)
+        with pytest.raises(TypeError, match=next(iter(kw))):
+            tied_head_distillation_loss(y, e, torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int32), **kw)
