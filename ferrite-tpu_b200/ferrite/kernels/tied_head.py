@@ -77,6 +77,9 @@ def _apply(y, e, loss, loss_and_grad, args, kw, logits_dtype):
         raise ValueError("y and the embedding must share a dtype")
     if logits_dtype not in (torch.float32, y.dtype):
         raise TypeError(f"logits of type {logits_dtype}: expected float32 or {y.dtype}")
+    if not (torch.is_grad_enabled() and (y.requires_grad or e.requires_grad)):  # an evaluation: the loss alone
+        with torch.no_grad():
+            return loss(gemm(y, e, trans_b=True, out_dtype=logits_dtype), *args, **kw)
     if y.dtype == torch.float16:
         return _TiedHeadLate.apply(y, e, loss, loss_and_grad, kw, logits_dtype, *args)
     return _TiedHead.apply(y, e, loss_and_grad, args, kw, logits_dtype)

@@ -59,3 +59,38 @@ def test_scales_of_the_logits_gradient_are_refused():
             tied_head_preference_loss(y, e, t, f, torch.tensor([0, 2, 4]), **kw)
         with pytest.raises(TypeError, match=next(iter(kw))):
             tied_head_distillation_loss(y, e, torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int32), **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["policy", "preference", "distill"])
+def test_no_gradient_is_computed_where_none_is_wanted(which):
+    """Under no_grad, and with operands that need none, the logits are all that is allocated; the results are the same."""
+    g = torch.Generator(device="cuda").manual_seed(17)
+    rows, d, vocab = 1024, 64, 32000
+    y = torch.randn(rows, d, device="cuda", generator=g).bfloat16()
+    e = (0.2 * torch.randn(vocab, d, device="cuda", generator=g)).bfloat16()
+    t, f = torch.randint(0, vocab, (rows,), device="cuda", generator=g), torch.full((rows,), -10.0, device="cuda")
+    off = torch.tensor([0, 500, rows], device="cuda")
+    v, i = torch.randn(rows, 8, device="cuda", generator=g), torch.randint(0, vocab, (rows, 8), device="cuda", generator=g)
+
+    def call(y, e):
+        return {"policy": lambda: tied_head_policy_loss(y, e, t, f, f, kl_coef=0.1, ref_logprobs=f), "preference": lambda: tied_head_preference_loss(y, e, t, f, off),
+                "distill": lambda: tied_head_distillation_loss(y, e, v, i)}[which]()
+
+    yg, eg = y.clone().requires_grad_(True), e.clone().requires_grad_(True)
+    want = call(yg, eg)
+    assert want.loss.requires_grad
+    kept = [o.detach().clone() for o in want]
+    del want
+    with torch.no_grad():
+        evaluated = lambda: call(yg, eg)  # noqa: E731
+        for fn in (evaluated, lambda: call(y, e)):
+            torch.cuda.synchronize()
+            before = torch.cuda.memory_allocated()
+            torch.cuda.reset_peak_memory_stats()
+            got = fn()
+            assert torch.cuda.max_memory_allocated() - before < rows * vocab * 5  # f32 logits; with a 16-bit gradient 6 bytes
+            assert not got.loss.requires_grad and all(torch.equal(a, b) for a, b in zip(got, kept))
+            del got
+    got = call(y, e)
+    assert not got.loss.requires_grad and torch.equal(got.loss, kept[0])
