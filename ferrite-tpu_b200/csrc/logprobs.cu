@@ -253,7 +253,8 @@ __global__ void __launch_bounds__(kPairThreads) pairs_kernel(Pairs a) {
     const float l = log1pf(expf(-fabsf(bh)));
     loss = (1.f - a.smooth) * (l + fmaxf(-bh, 0.f)) + a.smooth * (l + fmaxf(bh, 0.f));
     if (bh != bh) loss = bh;
-    dh = b * (1.f / (1.f + expf(-bh)) - (1.f - a.smooth));
+    // e sigma(bh) - (1 - e) sigma(-bh): of two terms near 1 (sigma(bh) - (1 - e)) the difference loses a settled pair's gradient
+    dh = b * (a.smooth / (1.f + expf(-bh)) - (1.f - a.smooth) / (1.f + expf(bh)));
   } else if (a.kind == 1) {  // squared
     const float q = h - 0.5f / b;
     loss = q * q;

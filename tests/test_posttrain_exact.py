@@ -13,6 +13,7 @@ import torch
 
 from ferrite import _native as nat
 from ferrite.kernels.policy_loss import policy_loss_and_grad
+from ferrite.kernels.preference_loss import preference_loss_and_grad
 
 U = 2.0**-24
 IGN = -100
@@ -88,3 +89,28 @@ def test_rows_whose_gradient_runs_behind(rows, vocab, dtype, c):
         b = min(rows, a + 50)
         assert all(torch.equal(p, q[a:b]) for p, q in zip(call(a, b), first))
     nat.device_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("smooth", [0.0, 0.01, 0.1])
+def test_preference_gradient_of_wide_margins(smooth):
+    """Pairs of one row each, margins from -20 to 20: d loss / d h = beta (e sigma(x) - (1 - e) sigma(-x)), x = beta h, to a
+    few roundings of it -- also where the pair is all but settled.  Relative bounds: x is off by its roundings and those
+    of two log-probabilities, which exp turns into a relative error; ten more roundings in the sigmoids."""
+    vocab, beta = 16, 0.1
+    margins = torch.cat([torch.linspace(-20, 20, 81), torch.tensor([30.0, 60.0, -60.0, 85.0])]).double()
+    pairs = len(margins)
+    x = torch.zeros(2 * pairs, vocab, device="cuda")
+    t = torch.zeros(2 * pairs, dtype=torch.long, device="cuda")
+    ref = torch.zeros(2 * pairs)
+    ref[1::2] = (margins / beta).float()  # h = -ref_chosen + ref_rejected
+    got = (ref[1::2].double() * float(np.float32(beta))).cuda()
+    out, grad = preference_loss_and_grad(x, t, ref.cuda(), torch.arange(2 * pairs + 1, device="cuda"), beta=beta, label_smoothing=smooth)
+    e = float(np.float32(smooth))
+    dh = float(np.float32(beta)) / pairs * (e * torch.sigmoid(got) - (1 - e) * torch.sigmoid(-got))
+    bound = (4 * tol(vocab) * beta + 4 * U * got.abs() + 16 * U)  # of each of the two terms
+    size = float(np.float32(beta)) / pairs * (e * torch.sigmoid(got) + (1 - e) * torch.sigmoid(-got))
+    for sign, rows in ((1.0, grad[0::2]), (-1.0, grad[1::2])):
+        for col, share in ((0, 15 / 16), (5, -1 / 16)):
+            err = (rows[:, col].double() - sign * share * dh).abs()
+            assert (err <= size * abs(share) * (bound + 2 * tol(vocab))).all(), (margins[int((err / size).argmax())], (err / size).max())
