@@ -100,6 +100,12 @@ def same_device(logits: torch.Tensor, *others: torch.Tensor | None) -> None:
             raise ValueError(f"tensors on {logits.device} and {t.device}: expected one device")
 
 
-def differentiable(logits: torch.Tensor) -> bool:
-    """Whether a call on these logits is to be recorded."""
-    return logits.requires_grad and torch.is_grad_enabled()
+def differentiable(logits: torch.Tensor, **others: torch.Tensor | None) -> bool:
+    """Whether a call on these logits is to be recorded.  The losses have a gradient in the logits only: where it
+    is recorded, another argument that asks for one is refused."""
+    if not (logits.requires_grad and torch.is_grad_enabled()):
+        return False
+    for name, t in others.items():
+        if t is not None and t.requires_grad:
+            raise ValueError(f"{name} requires a gradient, but the loss is differentiable in the logits only: pass it detached")
+    return True

@@ -81,15 +81,16 @@ class _Distillation(torch.autograd.Function):
 @nat.on_tensor_device
 def distillation_loss(logits, teacher_values, teacher_indices, weights=None, *, temperature: float = 1.0) -> DistillationLoss:
     """The distillation loss of ``logits [rows, vocab]`` against lists of a teacher's best tokens (see the
-    top of this file); ``loss`` is differentiable in the logits.
+    top of this file); ``loss`` is differentiable in the logits alone.
 
     teacher_values: ``[rows, top]`` f32, bf16 or f16 logits; teacher_indices: int32 or int64 tokens (an
     index at or above the vocabulary gives NaN; a token listed twice counts with both weights), at most
     1024 a row.  weights: one for each row, ``1 / rows`` by default; a row of weight zero is not read and
     gives zeros.
     """
+    recorded = _rows.differentiable(logits, teacher_values=teacher_values, weights=weights)
     values, indices, weights, temperature = _check(logits, teacher_values, teacher_indices, weights, temperature, None)
-    if not _rows.differentiable(logits):
+    if not recorded:
         return _launch(logits, values, indices, weights, temperature, None, None, 1.0)[0]
     return DistillationLoss(*_Distillation.apply(logits, values, indices, weights, temperature))
 

@@ -86,15 +86,16 @@ class _PolicyLoss(torch.autograd.Function):
 def policy_loss(logits, targets, old_logprobs, advantages, weights=None, *, ref_logprobs=None, clip_low: float = 0.2, clip_high: float = 0.2,
                 kl_coef: float = 0.0, entropy_coef: float = 0.0, temperature: float = 1.0, ignore_index: int = IGNORE_INDEX) -> PolicyLoss:
     """The clipped policy loss of ``logits [rows, vocab]`` (see the top of this file); ``loss`` is
-    differentiable in the logits, the per-row values are for monitoring.
+    differentiable in the logits alone, the per-row values are for monitoring.
 
     targets: int32 or int64, the tokens written.  old_logprobs, advantages, ref_logprobs, weights:
     one value for each row; weights default to ``1 / rows``.  A row of weight zero, or whose target is
     ``ignore_index``, is not read and gives zeros.
     """
+    recorded = _rows.differentiable(logits, old_logprobs=old_logprobs, advantages=advantages, weights=weights, ref_logprobs=ref_logprobs)
     targets, rest, temperature = _check(logits, targets, old_logprobs, advantages, weights, ref_logprobs, clip_low, clip_high, temperature, None)
     args = (logits, targets, rest, (float(clip_low), float(clip_high)), (float(kl_coef), float(entropy_coef)), temperature, int(ignore_index))
-    if not _rows.differentiable(logits):
+    if not recorded:
         return _launch(*args, None, None, 1.0)[0]
     return PolicyLoss(*_PolicyLoss.apply(*args))
 

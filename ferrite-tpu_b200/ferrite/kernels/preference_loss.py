@@ -100,16 +100,17 @@ class _Preference(torch.autograd.Function):
 def preference_loss(logits, targets, ref_logprobs, offsets, *, beta: float = 0.1, kind: str = "sigmoid", label_smoothing: float = 0.0,
                     average: bool = False, temperature: float = 1.0, ignore_index: int = IGNORE_INDEX) -> PreferenceLoss:
     """The preference loss of the packed ``logits [rows, vocab]`` (see the top of this file); ``loss`` is
-    differentiable in the logits.
+    differentiable in the logits alone.
 
     targets: int32 or int64; rows whose target is ``ignore_index`` (prompts, padding) are not read and
     count in no sequence.  ref_logprobs: the reference model's, one for each row.  offsets: int32 or
     int64 ``[2 pairs + 1]`` on the device, non-decreasing row numbers; rows outside every sequence get
     no gradient.  label_smoothing is the sigmoid loss's; the others do not use it.
     """
+    recorded = _rows.differentiable(logits, ref_logprobs=ref_logprobs)
     targets, ref, offsets, temperature = _check(logits, targets, ref_logprobs, offsets, beta, kind, label_smoothing, temperature, None)
     args = (logits, targets, ref, offsets, float(beta), kind, float(label_smoothing), bool(average), temperature, int(ignore_index))
-    if not _rows.differentiable(logits):
+    if not recorded:
         return _launch(*args, False, None, 1.0)[0]
     return PreferenceLoss(*_Preference.apply(*args))
 

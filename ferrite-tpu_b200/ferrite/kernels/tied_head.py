@@ -80,6 +80,8 @@ def _apply(y, e, loss, loss_and_grad, args, kw, logits_dtype):
     if not (torch.is_grad_enabled() and (y.requires_grad or e.requires_grad)):  # an evaluation: the loss alone
         with torch.no_grad():
             return loss(gemm(y, e, trans_b=True, out_dtype=logits_dtype), *args, **kw)
+    if any(isinstance(t, torch.Tensor) and t.requires_grad for t in (*args, *kw.values())):
+        raise ValueError("an argument requires a gradient, but the loss is differentiable in y and the embedding only: pass it detached")
     if y.dtype == torch.float16:
         return _TiedHeadLate.apply(y, e, loss, loss_and_grad, kw, logits_dtype, *args)
     return _TiedHead.apply(y, e, loss_and_grad, args, kw, logits_dtype)

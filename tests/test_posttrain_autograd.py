@@ -1,0 +1,61 @@
+"""What autograd may ask of the post-training losses, and what they refuse: they have a first derivative, in the logits."""
+
+import pytest
+import torch
+
+from ferrite.kernels.distillation import distillation_loss
+from ferrite.kernels.policy_loss import policy_loss
+from ferrite.kernels.preference_loss import preference_loss
+from ferrite.kernels.tied_head import tied_head_distillation_loss, tied_head_policy_loss, tied_head_preference_loss
+
+
+def _inputs(device, grad=True):
+    x = torch.randn(4, 64, device=device).requires_grad_(grad)
+    t = torch.zeros(4, dtype=torch.long, device=device)
+    f = torch.full((4,), -4.0, device=device)
+    off, v = torch.tensor([0, 2, 4], device=device), torch.zeros(4, 2, device=device)
+    return x, t, f, off, v, torch.zeros(4, 2, dtype=torch.int32, device=device)
+
+
+def _calls(x, t, f, off, v, i, y=None, e=None):
+    """(argument, call with that argument passed through ``on``)"""
+    calls = [
+        ("old_logprobs", lambda on: policy_loss(x, t, on(f), f)),
+        ("advantages", lambda on: policy_loss(x, t, f, on(f))),
+        ("weights", lambda on: policy_loss(x, t, f, f, on(f))),
+        ("ref_logprobs", lambda on: policy_loss(x, t, f, f, ref_logprobs=on(f), kl_coef=0.1)),
+        ("ref_logprobs", lambda on: preference_loss(x, t, on(f), off)),
+        ("teacher_values", lambda on: distillation_loss(x, on(v), i)),
+        ("weights", lambda on: distillation_loss(x, v, i, on(f))),
+    ]
+    if y is not None:
+        calls += [
+            ("argument", lambda on: tied_head_policy_loss(y, e, t, f, on(f))),
+            ("argument", lambda on: tied_head_policy_loss(y, e, t, f, f, ref_logprobs=on(f))),
+            ("argument", lambda on: tied_head_preference_loss(y, e, t, on(f), off)),
+            ("argument", lambda on: tied_head_distillation_loss(y, e, on(v), i)),
+        ]
+    return calls
+
+
+def _leaf(a):
+    return a.clone().requires_grad_(True)
+
+
+def test_other_arguments_that_ask_for_a_gradient_are_refused():
+    y, e = torch.zeros(4, 8, requires_grad=True), torch.zeros(64, 8)
+    for name, call in _calls(*_inputs("cpu"), y, e):
+        with pytest.raises(ValueError, match=f"{name} requires a gradient"):
+            call(_leaf)
+
+
+@pytest.mark.gpu
+def test_other_arguments_without_a_record_are_taken():
+    """Under no_grad, or where the logits are not recorded, nothing is lost; detached arguments are always taken."""
+    y, e = torch.randn(4, 64, device="cuda", requires_grad=True), torch.randn(64, 64, device="cuda")
+    for _, call in _calls(*_inputs("cuda"), y, e):
+        with torch.no_grad():
+            assert not call(_leaf).loss.requires_grad
+        assert call(lambda a: a).loss.requires_grad
+    for _, call in _calls(*_inputs("cuda", grad=False)):
+        assert not call(_leaf).loss.requires_grad
