@@ -9,6 +9,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from ferrite import _native as nat
 
@@ -100,10 +101,18 @@ def same_device(logits: torch.Tensor, *others: torch.Tensor | None) -> None:
             raise ValueError(f"tensors on {logits.device} and {t.device}: expected one device")
 
 
+def recorded(*tensors: torch.Tensor) -> bool:
+    """Whether autograd is to see a call on these: for a gradient, or for a forward-mode tangent (which its
+    function then refuses)."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return True
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def differentiable(logits: torch.Tensor, **others: torch.Tensor | None) -> bool:
     """Whether a call on these logits is to be recorded.  The losses have a gradient in the logits only: where it
     is recorded, another argument that asks for one is refused."""
-    if not (logits.requires_grad and torch.is_grad_enabled()):
+    if not recorded(logits):
         return False
     for name, t in others.items():
         if t is not None and t.requires_grad:

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import torch
 
+from ferrite.kernels import _rows
 from ferrite.kernels.distillation import DistillationLoss, distillation_loss, distillation_loss_and_grad
 from ferrite.kernels.matmul import gemm
 from ferrite.kernels.policy_loss import PolicyLoss, policy_loss, policy_loss_and_grad
@@ -77,7 +78,7 @@ def _apply(y, e, loss, loss_and_grad, args, kw, logits_dtype):
         raise ValueError("y and the embedding must share a dtype")
     if logits_dtype not in (torch.float32, y.dtype):
         raise TypeError(f"logits of type {logits_dtype}: expected float32 or {y.dtype}")
-    if not (torch.is_grad_enabled() and (y.requires_grad or e.requires_grad)):  # an evaluation: the loss alone
+    if not _rows.recorded(y, e):  # an evaluation: the loss alone
         with torch.no_grad():
             return loss(gemm(y, e, trans_b=True, out_dtype=logits_dtype), *args, **kw)
     if any(isinstance(t, torch.Tensor) and t.requires_grad for t in (*args, *kw.values())):

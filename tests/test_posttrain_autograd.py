@@ -2,8 +2,10 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from ferrite.kernels.distillation import distillation_loss
+from ferrite.kernels.logprobs import token_logprobs
 from ferrite.kernels.policy_loss import policy_loss
 from ferrite.kernels.preference_loss import preference_loss
 from ferrite.kernels.tied_head import tied_head_distillation_loss, tied_head_policy_loss, tied_head_preference_loss
@@ -59,3 +61,25 @@ def test_other_arguments_without_a_record_are_taken():
         assert call(lambda a: a).loss.requires_grad
     for _, call in _calls(*_inputs("cuda", grad=False)):
         assert not call(_leaf).loss.requires_grad
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_are_refused():
+    """A tangent raises whether or not the logits also ask for a gradient; a dual level without one changes nothing."""
+    x, t, f, off, v, i = _inputs("cuda", grad=False)
+    y, e = torch.randn(4, 64, device="cuda"), torch.randn(64, 64, device="cuda")
+    calls = [
+        (x, lambda z: token_logprobs(z, t)),
+        (x, lambda z: policy_loss(z, t, f, f)),
+        (x, lambda z: preference_loss(z, t, f, off)),
+        (x, lambda z: distillation_loss(z, v, i)),
+        (y, lambda z: tied_head_policy_loss(z, e, t, f, f)),
+        (e, lambda z: tied_head_policy_loss(y, z, t, f, f)),
+    ]
+    with fwd.dual_level():
+        for n, (at, call) in enumerate(calls):
+            call(at)
+            for grad in (False, True):
+                with pytest.raises(RuntimeError, match="jvp|forward AD"):
+                    call(fwd.make_dual(at.clone().requires_grad_(grad), torch.ones_like(at)))
+                    pytest.fail(f"call {n} dropped the tangent")
