@@ -118,3 +118,19 @@ def differentiable(logits: torch.Tensor, **others: torch.Tensor | None) -> bool:
         if t is not None and t.requires_grad:
             raise ValueError(f"{name} requires a gradient, but the loss is differentiable in the logits only: pass it detached")
     return True
+
+
+class _FirstOnly(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, grad, *sources):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("the losses over logits have no second derivative")
+
+
+def first_only(grad: torch.Tensor | None, *sources: torch.Tensor | None) -> torch.Tensor | None:
+    """A backward's result.  Where it is itself recorded (``create_graph``), what it depends on is named by ``sources``, so
+    that a second backward raises instead of passing it by as a constant."""
+    return grad if grad is None or not torch.is_grad_enabled() else _FirstOnly.apply(grad, *sources)

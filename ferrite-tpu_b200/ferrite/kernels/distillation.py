@@ -75,7 +75,7 @@ class _Distillation(torch.autograd.Function):
         # statistics and gradient in one launch, as in the policy loss
         logits, values, indices, weights = ctx.saved_tensors
         _, grad = _launch(logits, values, indices, weights, ctx.temperature, logits.dtype, _rows.upstream(g), 1.0)
-        return grad, None, None, None, None
+        return _rows.first_only(grad, logits, g), None, None, None, None
 
 
 @nat.on_tensor_device

@@ -64,7 +64,7 @@ class _TokenLogprobs(torch.autograd.Function):
         grad = logprobs_backward(
             logits, targets, stats, h, _rows.per_row(dlogp, rows, "dlogp"), _rows.per_row(dentropy, rows, "dentropy"), None, 1.0,
             ctx.temperature, ctx.ignore_index, logits.dtype)
-        return grad, None, None, None, None
+        return _rows.first_only(grad, logits, dlogp, dentropy), None, None, None, None
 
 
 @nat.on_tensor_device

@@ -79,7 +79,7 @@ class _PolicyLoss(torch.autograd.Function):
         # reading the logits for the gradient alone
         logits, targets, *rest = ctx.saved_tensors
         _, grad = _launch(logits, targets, rest, *ctx.args, logits.dtype, _rows.upstream(g), 1.0)
-        return grad, None, None, None, None, None, None
+        return _rows.first_only(grad, logits, g), None, None, None, None, None, None
 
 
 @nat.on_tensor_device

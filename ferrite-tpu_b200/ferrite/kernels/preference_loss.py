@@ -93,7 +93,7 @@ class _Preference(torch.autograd.Function):
     def backward(ctx, g, *_):
         logits, targets, stats, coef = ctx.saved_tensors
         grad = logprobs_backward(logits, targets, stats, None, coef, None, _rows.upstream(g), 1.0, ctx.temperature, ctx.ignore_index, logits.dtype)
-        return (grad, *([None] * 9))
+        return (_rows.first_only(grad, logits, g), *([None] * 9))
 
 
 @nat.on_tensor_device

@@ -37,8 +37,8 @@ class _TiedHead(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g, *_):
         y, e, dl = ctx.saved_tensors
-        dy, de = _products(ctx, dl, y, e)
-        return dy if dy is None else dy.mul_(g), de if de is None else de.mul_(g), None, None, None, None
+        dy, de = (_rows.first_only(d if d is None else d.mul_(g), y, e, g) for d in _products(ctx, dl, y, e))
+        return dy, de, None, None, None, None
 
 
 class _TiedHeadLate(torch.autograd.Function):
@@ -59,7 +59,8 @@ class _TiedHeadLate(torch.autograd.Function):
         y, e, logits, *rest = ctx.saved_tensors
         n = len(ctx.named)
         _, dl = ctx.loss_and_grad(logits, *rest[n:], grad_dtype=y.dtype, upstream=g, **dict(zip(ctx.named, rest[:n])), **ctx.kw)
-        return (*_products(ctx, dl, y, e), *([None] * (len(rest) - n + 4)))
+        dy, de = (_rows.first_only(d, y, e, g) for d in _products(ctx, dl, y, e))
+        return (dy, de, *([None] * (len(rest) - n + 4)))
 
 
 def _products(ctx, dl, y, e):

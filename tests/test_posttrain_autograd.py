@@ -83,3 +83,22 @@ def test_forward_mode_tangents_are_refused():
                 with pytest.raises(RuntimeError, match="jvp|forward AD"):
                     call(fwd.make_dual(at.clone().requires_grad_(grad), torch.ones_like(at)))
                     pytest.fail(f"call {n} dropped the tangent")
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    """Of a term with no second derivative in it the gradient's own would be all that is left, without a word."""
+    x, t, f, off, v, i = _inputs("cuda")
+    y, e = torch.randn(4, 64, device="cuda", requires_grad=True), torch.randn(64, 64, device="cuda")
+    losses = [
+        (x, lambda: token_logprobs(x, t).sum()),
+        (x, lambda: policy_loss(x, t, f, f).loss),
+        (x, lambda: preference_loss(x, t, f, off).loss),
+        (x, lambda: distillation_loss(x, v, i).loss),
+        (y, lambda: tied_head_policy_loss(y, e, t, f, f).loss),
+    ]
+    for n, (at, loss) in enumerate(losses):
+        (g,) = torch.autograd.grad(loss(), at, create_graph=True)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            (g.pow(2).sum() + at.sum()).backward()
+            pytest.fail(f"loss {n}: the second derivative was dropped")
