@@ -50,18 +50,19 @@ __device__ __forceinline__ void store_at(TO* p, const float (&d)[N], bool vec) {
 }
 
 // What stands for the elements of vectors past a row's end: nothing of the sums.  -inf, but in 0 * y
-// where the entropy is summed -1e30; f16 has none that is small enough for every temperature.
+// where the entropy is summed -1e30; f16 has none that is small enough for every temperature, and takes the vectors
+// of a piece that is not whole one by one, with the entropy or without (a row's s must not depend on that).
 template <typename T, bool ENT>
 struct Pad {
-  static constexpr bool kThere = !ENT || !std::is_same_v<T, __half>;
-  static constexpr uint32_t kBits = std::is_same_v<T, float>    ? (ENT ? 0xf149f2cau : 0xff800000u)
-                                    : std::is_same_v<T, __half> ? 0xfc00fc00u
-                                                                : (ENT ? 0xf149f149u : 0xff80ff80u);
+  static constexpr bool kThere = !std::is_same_v<T, __half>;
+  static constexpr uint32_t kBits = std::is_same_v<T, float> ? (ENT ? 0xf149f2cau : 0xff800000u) : (ENT ? 0xf149f149u : 0xff80ff80u);
   static __device__ __forceinline__ uint4 vector() { return make_uint4(kBits, kBits, kBits, kBits); }
 };
-// Adds Q vectors to a state by one check of their sums; false, and nothing added, if they are not usual.
+// Adds Q vectors to a state by one check of their sum.  What is left to do, vector by vector: nothing; their
+// part of u (dot_masked); or all of it (push).
+enum class Left { kNothing, kDot, kAll };
 template <bool ENT, typename T, int Q>
-__device__ __forceinline__ bool push_usual(State& st, float nc, const uint4 (&raw)[Q], const Pairs2& kk) {
+__device__ __forceinline__ Left push_usual(State& st, float nc, const uint4 (&raw)[Q], const Pairs2& kk) {
   uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
@@ -70,10 +71,18 @@ __device__ __forceinline__ bool push_usual(State& st, float nc, const uint4 (&ra
     sum_usual<ENT>(s2, u2, vals, nc, kk);
   }
   const float s = f2_lo(s2) + f2_hi(s2), u = ENT ? f2_lo(u2) + f2_hi(u2) : 0.f;
-  if (!usual<ENT>(s, u)) return false;
+  if (!usual(s)) return Left::kAll;
   st.s += s;
-  if constexpr (ENT) st.u += u;
-  return true;
+  if constexpr (ENT) {
+    if (u != u) return Left::kDot;
+    st.u += u;
+  }
+  return Left::kNothing;
+}
+template <bool ENT, int N>
+__device__ __forceinline__ void push_left(State& st, float& nc, const float (&x)[N], const RowIn& in, const Pairs2& kk, Left left) {
+  if (ENT && left == Left::kDot) st.u += dot_masked(x, nc, in);
+  else push<ENT>(st, nc, x, in, kk);
 }
 
 // --------------------------------------------------------------------------
@@ -133,19 +142,19 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
         const TI* at = x + cut.head + v * N;
         const int left = cut.nv - v;
         uint4 raw[kShortVecs];
-        bool by_one = !P::kThere && (kShortVecs - 1) * 32 >= left;
-        if (!by_one) {
+        Left todo = Left::kAll;
+        if (P::kThere || (kShortVecs - 1) * 32 < left) {
 #pragma unroll
-          for (int q = 0; q < kShortVecs; ++q) raw[q] = q * 32 < left ? ld_v4(at + q * 32 * N) : P::vector();
-          by_one = !push_usual<Op::kEnt, TI>(st, nc, raw, kk);
+          for (int q = 0; q < kShortVecs; ++q) raw[q] = !P::kThere || q * 32 < left ? ld_v4(at + q * 32 * N) : P::vector();
+          todo = push_usual<Op::kEnt, TI>(st, nc, raw, kk);
         }
-        if (by_one) {
+        if (todo != Left::kNothing) {
 #pragma unroll 1
           for (int q = 0; q < kShortVecs; ++q)
             if (q * 32 < left) {
               float vals[N];
               unpack16<TI>(ld_v4(at + q * 32 * N), vals);
-              push<Op::kEnt>(st, nc, vals, in, kk);
+              push_left<Op::kEnt>(st, nc, vals, in, kk, todo);
             }
         }
       }
@@ -551,7 +560,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
       for (int c = c0; c < row.chunks; c += kGroups) {
         (void)mbar_wait(&sh.full[at.at], at.parity, abort, 209);
         const uint4* v = reinterpret_cast<const uint4*>(ring + (size_t)at.at * kChunk) + gtid;
-        bool by_one = true;
+        Left todo = Left::kAll;
         if (P::kThere || (kVecPer - 1) * kGroup < left) {  // all of the thread's vectors at once
           uint4 raw[kVecPer];
 #pragma unroll
@@ -559,15 +568,15 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
             raw[q] = v[q * kGroup];  // past the row's end: whatever the chunk holds
             if (P::kThere && q * kGroup >= left) raw[q] = P::vector();
           }
-          by_one = !push_usual<Op::kEnt, TI>(st, nc, raw, kk);
+          todo = push_usual<Op::kEnt, TI>(st, nc, raw, kk);
         }
-        if (by_one) {
+        if (todo != Left::kNothing) {
 #pragma unroll 1
           for (int q = 0; q < kVecPer; ++q)
             if (q * kGroup < left) {
               float vals[N];
               unpack16<TI>(v[q * kGroup], vals);
-              push<Op::kEnt>(st, nc, vals, in, kk);
+              push_left<Op::kEnt>(st, nc, vals, in, kk, todo);
             }
         }
         __syncwarp();

@@ -145,7 +145,8 @@ struct Pairs2 {
 };
 
 // Sums of the usual values: per pair of elements two packed fma (y), two ex2 and packed adds.  They
-// count only if usual() holds of them; otherwise the elements go through push_any.
+// count only if usual() holds of s; otherwise the elements go through push_any.  u then is right too, or NaN from an
+// e of 0 times a y of -inf (masked columns, a row's padding): dot_masked has it without those.
 template <bool ENT, int N>
 __device__ __forceinline__ void sum_usual(uint64_t& s2, uint64_t& u2, const float (&x)[N], float nc, const Pairs2& kk) {
   const uint64_t c2 = f2_make(nc, nc);
@@ -155,12 +156,21 @@ __device__ __forceinline__ void sum_usual(uint64_t& s2, uint64_t& u2, const floa
     const uint64_t y2 = f2_fma(x2, kk.k_rest, f2_fma(x2, kk.k_hi, c2));
     const uint64_t e2 = f2_make(ex2_approx(f2_lo(y2)), ex2_approx(f2_hi(y2)));
     s2 = f2_add(s2, e2);
-    if constexpr (ENT) u2 = f2_fma(e2, y2, u2);  // -inf: 0 * -inf = NaN, and not usual
+    if constexpr (ENT) u2 = f2_fma(e2, y2, u2);
   }
 }
-template <bool ENT>
-__device__ __forceinline__ bool usual(float s, float u) {
-  return ENT ? fmaf(fabsf(u), 1.f / 128.f, s) < kHuge : s < kHuge;  // false for NaN
+// Whether a sum of usual values counts (false for NaN).  By s alone: how a row's s is put together, and so its
+// log-probability to the last bit, must not depend on whether u is asked for.
+__device__ __forceinline__ bool usual(float s) { return s < kHuge; }
+template <int N>
+__device__ __forceinline__ float dot_masked(const float (&x)[N], float nc, const RowIn& in) {
+  float u = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float y = fmaf(x[i], in.k_rest, fmaf(x[i], in.k_hi, nc));
+    u = fmaf(ex2_approx(y), fmaxf(y, -1000.f), u);
+  }
+  return u;
 }
 
 // Adds N elements to a state; nc = minus_c(st.m), kept up to date.
@@ -169,10 +179,14 @@ __device__ __forceinline__ void push(State& st, float& nc, const float (&x)[N], 
   if constexpr (N % 2 == 0) {
     uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
     sum_usual<ENT>(s2, u2, x, nc, kk);
-    const float s = f2_lo(s2) + f2_hi(s2), u = ENT ? f2_lo(u2) + f2_hi(u2) : 0.f;
-    if (usual<ENT>(s, u)) {
+    const float s = f2_lo(s2) + f2_hi(s2);
+    float u = ENT ? f2_lo(u2) + f2_hi(u2) : 0.f;
+    if (usual(s)) {
+      if constexpr (ENT) {
+        if (u != u) u = dot_masked(x, nc, in);
+        st.u += u;
+      }
       st.s += s;
-      if constexpr (ENT) st.u += u;
       return;
     }
   }

@@ -12,7 +12,8 @@ import pytest
 import torch
 
 from ferrite import _native as nat
-from ferrite.kernels.policy_loss import policy_loss_and_grad
+from ferrite.kernels.logprobs import token_logprobs
+from ferrite.kernels.policy_loss import policy_loss, policy_loss_and_grad
 from ferrite.kernels.preference_loss import preference_loss_and_grad
 
 U = 2.0**-24
@@ -114,3 +115,48 @@ def test_preference_gradient_of_wide_margins(smooth):
         for col, share in ((0, 15 / 16), (5, -1 / 16)):
             err = (rows[:, col].double() - sign * share * dh).abs()
             assert (err <= size * abs(share) * (bound + 2 * tol(vocab))).all(), (margins[int((err / size).argmax())], (err / size).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,dtype", [(40, 1003, "f16"), (40, 1000, "bf16"), (40, 1004, "f32"), (40, 7000, "f16"), (700, 8200, "f16"), (700, 12000, "bf16"), (40, 32008, "f16"), (40, 32000, "bf16"), (40, 50304, "f32"), (10, 131080, "f16")])
+@pytest.mark.parametrize("hide", ["nothing", "inf", "lowest"])
+@pytest.mark.parametrize("tau", [1.0, 0.7, 3000.0])
+def test_logprobs_have_the_same_bits_from_every_operator(rows, vocab, dtype, hide, tau):
+    """Log-probabilities alone, with entropies, and those of the policy loss, with and without a gradient and a bonus:
+    one row, one result -- masked columns and rows that end inside a vector among them."""
+    ld = -(-vocab // 8) * 8
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = (3 * torch.randn(rows, ld, device="cuda", generator=g)).to(TORCH[dtype])[:, :vocab]
+    t = torch.randint(0, vocab // 2, (rows,), device="cuda", generator=g)
+    if hide != "nothing":
+        low = -float("inf") if hide == "inf" else torch.finfo(TORCH[dtype]).min
+        x[:, vocab - vocab // 50 :] = low
+        x[::2, vocab // 2 :][torch.rand(len(x[::2]), vocab - vocab // 2, device="cuda", generator=g) < 0.1] = low
+    alone = token_logprobs(x, t, temperature=tau)
+    assert torch.isfinite(alone).all()
+    both, _ = token_logprobs(x, t, temperature=tau, entropy=True)
+    assert torch.equal(alone, both)
+    f = torch.randn(rows, device="cuda", generator=g)
+    assert torch.equal(policy_loss(x, t, alone, f, temperature=tau).logprobs, alone)
+    for c in (0.0, 0.01):
+        out, _ = policy_loss_and_grad(x, t, alone, f, entropy_coef=c, temperature=tau)
+        assert torch.equal(out.logprobs, alone)
+    off = torch.tensor([0, rows // 2, rows], device="cuda")
+    assert torch.equal(preference_loss_and_grad(x, t, alone, off, temperature=tau)[0].logprobs, alone)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [1003, 8203, 50257])
+@pytest.mark.parametrize("tau", [1.0, 2.0, 300.0, 3000.0, 1e5])
+@pytest.mark.parametrize("level", [0.0, -20000.0, -65000.0, 60000.0])
+def test_f16_rows_that_end_inside_a_vector(vocab, tau, level):
+    """What stands for the elements past a row's end counts for nothing, whatever the temperature and the logits' level."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = (level + 3 * max(1.0, tau / 30) * torch.randn(6, vocab, device="cuda", generator=g)).clamp(-65504, 65504).half()
+    t = torch.randint(0, vocab, (6,), device="cuda", generator=g)
+    lp, h = token_logprobs(x, t, temperature=tau, entropy=True)
+    want, p, wh = softmax64(x, tau)
+    want = want.gather(1, t[:, None])[:, 0]
+    # at a level of 65000 k m is rounded to 2^-8 / tau: one number for a row, so it does not show in log p or H
+    assert ((lp - want).abs() <= tol(vocab) * (1 + want.abs())).all()
+    assert ((h - wh).abs() <= 2 * tol(vocab) * (2 + wh + np.log(vocab))).all()
