@@ -14,7 +14,7 @@ constexpr int kMaxTop = 1024;
 constexpr int kSeenWords = 256;
 
 struct Distill {
-  static constexpr bool kEnt = false, kGradEnt = false, kHasStats = false, kList = true, kForwardOnly = false;
+  static constexpr bool kLogp = false, kEnt = false, kGradEnt = false, kHasStats = false, kList = true, kForwardOnly = false;
   const void* values;   // [rows, top] teacher logits
   const void* indices;  // [rows, top]
   int64_t ld_list;

@@ -18,9 +18,22 @@ __device__ __forceinline__ float logit_at(const TI* x, int64_t t, int64_t n) {
   return t >= 0 && t < n ? DT<TI>::to_f(x[t]) : __int_as_float(0x7fc00000);
 }
 
+// The same by a whole warp, and a base: the largest of the 32 logits around it, which come with it.
+template <typename TI>
+__device__ __forceinline__ float logit_and_base(const TI* x, int64_t t, const RowIn& in, float& base) {
+  const int lane = threadIdx.x & 31;
+  const int64_t i = (t & ~(int64_t)31) + lane;
+  const float v = t >= 0 && t < in.vocab && i < in.vocab ? DT<TI>::to_f(x[i]) : __int_as_float(0x7fc00000);
+  float m = v;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  base = base_of(m, in);
+  return __shfl_sync(0xffffffffu, v, (int)(t & 31));
+}
+
 template <bool ENT>
 struct LogprobsFwd {
-  static constexpr bool kEnt = ENT, kGradEnt = false, kHasStats = false, kList = false, kForwardOnly = true;
+  static constexpr bool kLogp = true, kEnt = ENT, kGradEnt = false, kHasStats = false, kList = false, kForwardOnly = true;
   Targets t;
   float* logp;
   float* entropy;
@@ -41,9 +54,10 @@ struct LogprobsFwd {
   }
   template <typename TI>
   __device__ float prep(int64_t, const Pre& p, const TI* x, const RowIn& in, char* slot) const {
-    const float xt = logit_at(x, p.t, in.vocab);
+    float base;
+    const float xt = logit_and_base(x, p.t, in, base);
     if ((threadIdx.x & 31) == 0) reinterpret_cast<Row*>(slot)->xt = xt;
-    return base_of(xt, in);
+    return base;
   }
   __device__ Coef finish(int64_t, const Norm&, const RowIn&, float, char*) const { return Coef{}; }
   __device__ void results(int64_t r, const Norm& w, const RowIn& in, char* slot) const {
@@ -57,7 +71,7 @@ struct LogprobsFwd {
 
 template <bool ENT>
 struct LogprobsBwd {
-  static constexpr bool kEnt = false, kGradEnt = ENT, kHasStats = true, kList = false, kForwardOnly = false;
+  static constexpr bool kLogp = true, kEnt = false, kGradEnt = ENT, kHasStats = true, kList = false, kForwardOnly = false;
   Targets t;
   const float2* stats;
   const float* entropy;   // ENT: the forward's
@@ -84,7 +98,7 @@ struct LogprobsBwd {
     w.a = p.t >= 0 && p.t < in.vocab ? (dlogp ? dlogp[r] : 0.f) : __int_as_float(0x7fc00000);
     w.b = 0.f;
     if constexpr (ENT) {
-      w.w.u = w.w.s * (log2f(w.w.s) - entropy[r] * kLog2e);
+      w.w.mean = log2f(w.w.s) - entropy[r] * kLog2e;
       w.b = dentropy[r];
     }
     w.t = p.t;
@@ -102,7 +116,7 @@ struct LogprobsBwd {
 // ENT: the entropy bonus takes part in the gradient (its value is always written).
 template <bool ENT>
 struct Policy {
-  static constexpr bool kEnt = true, kGradEnt = ENT, kHasStats = false, kList = false, kForwardOnly = false;
+  static constexpr bool kLogp = true, kEnt = true, kGradEnt = ENT, kHasStats = false, kList = false, kForwardOnly = false;
   Targets t;
   const float* old_logp;
   const float* adv;
@@ -131,9 +145,10 @@ struct Policy {
   }
   template <typename TI>
   __device__ float prep(int64_t r, const Pre& p, const TI* x, const RowIn& in, char* slot) const {
-    const float xt = logit_at(x, p.t, in.vocab);
+    float base;
+    const float xt = logit_and_base(x, p.t, in, base);
     if ((threadIdx.x & 31) == 0) *reinterpret_cast<Row*>(slot) = Row{p.t, p.w, xt, old_logp[r], adv[r], ref ? ref[r] : 0.f};
-    return base_of(xt, in);
+    return base;
   }
   struct Step {
     float logp, ratio, plain, bounded, em;  // em = exp(ref - logp) - 1

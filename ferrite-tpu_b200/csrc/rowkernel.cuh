@@ -3,6 +3,7 @@
 //
 // An Op provides
 //   kEnt        the sum of e * y is needed (the entropy's value, or its gradient)
+//   kLogp       log p of single logits and the entropy are asked for: sums against a high base
 //   kGradEnt    the gradient has the entropy's term
 //   kHasStats   the row's state is an input: no first pass
 //   kList       the gradient has more single entries than the target's
@@ -58,31 +59,27 @@ struct Pad {
   static constexpr uint32_t kBits = std::is_same_v<T, float> ? (ENT ? 0xf149f2cau : 0xff800000u) : (ENT ? 0xf149f149u : 0xff80ff80u);
   static __device__ __forceinline__ uint4 vector() { return make_uint4(kBits, kBits, kBits, kBits); }
 };
-// Adds Q vectors to a state by one check of their sum.  What is left to do, vector by vector: nothing; their
-// part of u (dot_masked); or all of it (push).
+// Adds Q vectors to a state by one check of their sums.  What is left to do, vector by vector: nothing; their
+// part of u; or all of it.
 enum class Left { kNothing, kDot, kAll };
-template <bool ENT, typename T, int Q>
+template <class Op, typename T, int Q>
 __device__ __forceinline__ Left push_usual(State& st, float nc, const uint4 (&raw)[Q], const Pairs2& kk) {
   uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
     float vals[16 / sizeof(T)];
     unpack16<T>(raw[q], vals);
-    sum_usual<ENT>(s2, u2, vals, nc, kk);
+    sum_usual<Op::kEnt>(s2, u2, vals, nc, kk);
   }
-  const float s = f2_lo(s2) + f2_hi(s2), u = ENT ? f2_lo(u2) + f2_hi(u2) : 0.f;
-  if (!usual(s)) return Left::kAll;
+  const float s = f2_lo(s2) + f2_hi(s2), u = Op::kEnt ? f2_lo(u2) + f2_hi(u2) : 0.f;
+  if (usual<Op::kLogp>(Op::kEnt ? fmaf(u, 0.f, s) : s)) {  // s, or NaN where u is
+    st.s += s;
+    if constexpr (Op::kEnt) st.u += u;
+    return Left::kNothing;
+  }
+  if (!Op::kEnt || !usual<Op::kLogp>(s)) return Left::kAll;
   st.s += s;
-  if constexpr (ENT) {
-    if (u != u) return Left::kDot;
-    st.u += u;
-  }
-  return Left::kNothing;
-}
-template <bool ENT, int N>
-__device__ __forceinline__ void push_left(State& st, float& nc, const float (&x)[N], const RowIn& in, const Pairs2& kk, Left left) {
-  if (ENT && left == Left::kDot) st.u += dot_masked(x, nc, in);
-  else push<ENT>(st, nc, x, in, kk);
+  return Left::kDot;
 }
 
 // --------------------------------------------------------------------------
@@ -146,7 +143,8 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
         if (P::kThere || (kShortVecs - 1) * 32 < left) {
 #pragma unroll
           for (int q = 0; q < kShortVecs; ++q) raw[q] = !P::kThere || q * 32 < left ? ld_v4(at + q * 32 * N) : P::vector();
-          todo = push_usual<Op::kEnt, TI>(st, nc, raw, kk);
+          if constexpr (Op::kLogp) raise<Op::kEnt>(st, nc, max_of<TI>(raw), in);
+          todo = push_usual<Op, TI>(st, nc, raw, kk);
         }
         if (todo != Left::kNothing) {
 #pragma unroll 1
@@ -154,13 +152,13 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
             if (q * 32 < left) {
               float vals[N];
               unpack16<TI>(ld_v4(at + q * 32 * N), vals);
-              push_left<Op::kEnt>(st, nc, vals, in, kk, todo);
+              push<Op::kEnt, Op::kLogp>(st, nc, vals, in, kk, todo == Left::kDot);
             }
         }
       }
       if (edge >= 0) {
         const float one[1] = {edge_x};
-        push<Op::kEnt>(st, nc, one, in, kk);
+        push<Op::kEnt, Op::kLogp>(st, nc, one, in, kk);
       }
       __syncwarp();
       w = normalise<Op::kEnt>(warp_merge<Op::kEnt>(st, in), in);
@@ -487,7 +485,8 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
       // Fetches row r into one of the helper's two slots and announces its base.
       auto fetch = [&](int which) {
         const int64_t at = nth(r);
-        const float base = op.prep(at, op.pre(at), static_cast<const TI*>(in.logits) + at * in.ld, in, slots + (2 * h + which) * slot_bytes);
+        const TI* x = static_cast<const TI*>(in.logits) + at * in.ld;
+        const float base = op.prep(at, op.pre(at), x, in, slots + (2 * h + which) * slot_bytes);
         __syncwarp();
         if (kSums && lane == 0) {
           sh.base[h] = base;
@@ -568,7 +567,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
             raw[q] = v[q * kGroup];  // past the row's end: whatever the chunk holds
             if (P::kThere && q * kGroup >= left) raw[q] = P::vector();
           }
-          todo = push_usual<Op::kEnt, TI>(st, nc, raw, kk);
+          todo = push_usual<Op, TI>(st, nc, raw, kk);
         }
         if (todo != Left::kNothing) {
 #pragma unroll 1
@@ -576,7 +575,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
             if (q * kGroup < left) {
               float vals[N];
               unpack16<TI>(v[q * kGroup], vals);
-              push_left<Op::kEnt>(st, nc, vals, in, kk, todo);
+              push<Op::kEnt, Op::kLogp>(st, nc, vals, in, kk, todo == Left::kDot);
             }
         }
         __syncwarp();
@@ -586,7 +585,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
       }
       if (edge >= 0) {
         const float one[1] = {edge_x};
-        push<Op::kEnt>(st, nc, one, in, kk);
+        push<Op::kEnt, Op::kLogp>(st, nc, one, in, kk);
       }
       __syncwarp();
       st = warp_merge<Op::kEnt>(st, in);

@@ -8,11 +8,13 @@
 //   logp_i = ln2 (y_i - log2 s),   H = ln2 (log2 s - u / s),   p_i = e_i / s.
 // A row's state is (m, s, u): it is built in one pass and merged pairwise.  m is a base, not the
 // maximum: 2^y keeps its precision over the whole exponent range, so any logit of the row's upper
-// part serves, and the sums are checked instead -- a sum that reaches 2^80 (an element 2^80 above the
-// base) is redone against the largest element.  No maximum is taken per element, and no rescaling
-// runs in the usual case.  The base is the logit of the target (or of the teacher's first token),
-// whose own term is then 1 without rounding.  All of it is f32; only the gradient is rounded, once,
-// on store.
+// part serves, and the sums are checked instead -- one that is too high is redone against the largest
+// element.  No maximum is taken per element, and no rescaling runs in the usual case.  Too high is 2^10 where
+// log p and the entropy are asked for: log2 s and u / s both grow with the distance of the base from
+// the row's upper part, the entropy is their difference, and what it loses is a few roundings of
+// that distance.  So that few sums are redone, the base there is the largest of the 32 logits that are fetched with the
+// target's.  Elsewhere (distillation) it is 2^80, and the base is the student's logit at a teacher's token.  The base's own
+// term is 1 without rounding.  All of it is f32; only the gradient is rounded, once, on store.
 //
 // y_i is K x_i - c with c = k m rounded -- one number for every term of s and for logp, so that its
 // rounding cancels -- and K is carried to more than f32: the rounding of k alone would shift every
@@ -37,7 +39,7 @@ namespace rowloss {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kBig = 65536.f;   // |k m| above this: y is k (x - m)
-constexpr float kHuge = 0x1p80f;  // a sum above this is redone against the maximum
+constexpr float kHigh = 0x1p10f, kHuge = 0x1p80f;  // sums above this (an Op's) are redone against the maximum
 
 // (m, s, u): the base, sum of e and sum of e * y of the elements seen so far.
 struct State {
@@ -76,7 +78,7 @@ __device__ __forceinline__ float base_of(float x, const RowIn& in) { return is_b
 // y of base m1 against base m2 >= m1 (neither -inf): the log2 of the factor that takes sums over
 // to the new base.
 __device__ __forceinline__ float base_step(float m1, float m2, const RowIn& in) {
-  const float c1 = m1 * in.k, c2 = m2 * in.k;
+  const float c1 = __fmul_rn(m1, in.k), c2 = __fmul_rn(m2, in.k);
   if (!is_big(c1)) return !is_big(c2) ? c1 - c2 : -(fmaf(m2, in.k, -c1) + m2 * in.k_lo);
   return !is_big(c2) ? fmaf(m1, in.k, -c2) + m1 * in.k_lo : (m1 - m2) * in.k;
 }
@@ -90,7 +92,7 @@ __device__ __forceinline__ void rebase(State& st, float m, const RowIn& in) {
   }
   const float d = base_step(st.m, m, in), f = ex2_approx(d);
   if constexpr (ENT) st.u = f > 0.f && st.s != 0.f ? f * fmaf(st.s, d, st.u) : 0.f;
-  st.s *= f;
+  st.s = __fmul_rn(st.s, f);  // (never one fma with what is added to it: a row's s has the same bits in every kernel)
   st.m = m;
 }
 
@@ -134,7 +136,7 @@ __device__ __forceinline__ void push_any(State& st, const float (&x)[N], const R
 
 // -k m for the usual values' form of y, or NaN where the base is big (every sum then fails its check).
 __device__ __forceinline__ float minus_c(float m, const RowIn& in) {
-  const float c = m * in.k;
+  const float c = __fmul_rn(m, in.k);
   return is_big(c) ? __int_as_float(0x7fc00000) : -c;
 }
 
@@ -161,7 +163,10 @@ __device__ __forceinline__ void sum_usual(uint64_t& s2, uint64_t& u2, const floa
 }
 // Whether a sum of usual values counts (false for NaN).  By s alone: how a row's s is put together, and so its
 // log-probability to the last bit, must not depend on whether u is asked for.
-__device__ __forceinline__ bool usual(float s) { return s < kHuge; }
+template <bool LOGP>
+__device__ __forceinline__ bool usual(float s) {
+  return s < (LOGP ? kHigh : kHuge);
+}
 template <int N>
 __device__ __forceinline__ float dot_masked(const float (&x)[N], float nc, const RowIn& in) {
   float u = 0.f;
@@ -173,43 +178,60 @@ __device__ __forceinline__ float dot_masked(const float (&x)[N], float nc, const
   return u;
 }
 
-// Adds N elements to a state; nc = minus_c(st.m), kept up to date.
-template <bool ENT, int N>
-__device__ __forceinline__ void push(State& st, float& nc, const float (&x)[N], const RowIn& in, const Pairs2& kk) {
+// Moves the base up to cm, the maximum of what is added next; nc = minus_c(st.m), kept up to date.  What stands for
+// elements past a row's end (down to -1e30) is no base.
+template <bool ENT>
+__device__ __forceinline__ bool raise(State& st, float& nc, float cm, const RowIn& in) {
+  if (!(cm > st.m && cm > -9e29f)) return false;
+  rebase<ENT>(st, cm, in);
+  nc = minus_c(cm, in);
+  return true;
+}
+// Adds N elements to a state; `dot`: to its u alone.
+template <bool ENT, bool LOGP, int N>
+__device__ __forceinline__ void push(State& st, float& nc, const float (&x)[N], const RowIn& in, const Pairs2& kk, bool dot = false) {
   if constexpr (N % 2 == 0) {
-    uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
-    sum_usual<ENT>(s2, u2, x, nc, kk);
-    const float s = f2_lo(s2) + f2_hi(s2);
-    float u = ENT ? f2_lo(u2) + f2_hi(u2) : 0.f;
-    if (usual(s)) {
-      if constexpr (ENT) {
-        if (u != u) u = dot_masked(x, nc, in);
-        st.u += u;
+    for (bool again = true; again;) {
+      uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
+      sum_usual<ENT>(s2, u2, x, nc, kk);
+      const float s = f2_lo(s2) + f2_hi(s2);
+      float u = ENT ? f2_lo(u2) + f2_hi(u2) : 0.f;
+      if (usual<LOGP>(s)) {
+        if constexpr (ENT) {
+          if (u != u) u = dot_masked(x, nc, in);
+          st.u += u;
+        }
+        if (!ENT || !dot) st.s += s;
+        return;
       }
-      st.s += s;
-      return;
+      float cm = x[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) cm = fmaxf(cm, x[i]);
+      again = raise<ENT>(st, nc, cm, in);
     }
   }
   push_any<ENT>(st, x, in);
   nc = minus_c(st.m, in);
 }
 
-// A finished row: base (c, or m where big), s, u.
+// A finished row: base (c, or m where big), s, and the mean of y, u / s.
 struct Norm {
-  float base, s, u;
+  float base, s, mean;
   int big;
 };
 // Moves the power of two of s into the base, exactly: c2 = c + j is rounded, and what the rounding
 // left goes back into s (2^err by its series: |err| <= 2^-7).
 template <bool ENT>
 __device__ __forceinline__ Norm normalise(const State& st, const RowIn& in) {
-  const float c = st.m * in.k;
-  if (is_big(c) || !(st.s < INFINITY)) return Norm{is_big(c) ? st.m : c, st.s, st.u, is_big(c)};
+  const float c = __fmul_rn(st.m, in.k);
+  if (is_big(c) || !(st.s < INFINITY)) return Norm{is_big(c) ? st.m : c, st.s, ENT ? st.u / st.s : 0.f, is_big(c)};
   const uint32_t bits = __float_as_uint(st.s);
   const float l = (float)((int)(bits >> 23) - 127), f = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);  // s = 2^l f
   const float c2 = c + l, b = c2 - c, err = (c - (c2 - b)) + (l - b);  // c + l = c2 + err
   const float t = err * kLn2, s = fmaf(f, fmaf(0.5f * t, t, t), f);
-  return Norm{c2, s, ENT ? s * (st.u / st.s - l + err) : 0.f, 0};
+  if constexpr (!ENT) return Norm{c2, s, 0.f, 0};
+  const float inv = __fdividef(1.f, st.s), q = st.u * inv, rest = fmaf(-q, st.s, st.u) * inv;  // u / s = q + rest
+  return Norm{c2, s, (q - l) + (rest + err), 0};
 }
 __device__ __forceinline__ float y_of(float x, const Norm& w, const RowIn& in) {
   return w.big ? (x - w.base) * in.k : fmaf(x, in.k_rest, fmaf(x, in.k_hi, -w.base));
@@ -222,13 +244,16 @@ __device__ __forceinline__ float y_of(float x, const Norm& w, const RowIn& in) {
 // log p is then off by 3.4e-8 at most on average, 6e-9 at tau 1 (tau 0.7 to 2, 256 to 131072 columns).
 constexpr float kEx2Below = -5.1e-8f, kEx2Above = 3.4e-8f;
 __device__ __forceinline__ float logp_of(float xt, const Norm& w, const RowIn& in) {
-  const double k = (double)in.k + (double)in.k_lo;
-  const double y = (w.big ? (double)(xt - w.base) * k : (double)xt * k - (double)w.base) - (double)log2f(w.s);
+  const double k = (double)in.k + (double)in.k_lo, l = (double)log2f(w.s);
+  const double y = w.big ? fma((double)(xt - w.base), k, -l) : fma((double)xt, k, -(double)w.base) - l;
   const float p = ex2_approx((float)y), ahead = (float)y + log2f((float)in.vocab);
   const float below = 1.f / (1.f + ex2_approx(fminf(3.f - 2.f / 3.f * ahead, 100.f)));
   return (float)(y * 0.6931471805599453 + (double)(fmaf(below, kEx2Below - kEx2Above, kEx2Above) * (1.f - p)));
 }
-__device__ __forceinline__ float entropy_of(const Norm& w) { return (log2f(w.s) - w.u / w.s) * kLn2; }
+__device__ __forceinline__ float entropy_of(const Norm& w) {
+  const float h = (log2f(w.s) - w.mean) * kLn2;
+  return h < 0.f ? 0.f : h;
+}
 
 // 16 bytes of T as floats.
 template <typename T>
@@ -246,6 +271,24 @@ __device__ __forceinline__ void unpack16(const uint4& v, float (&f)[16 / sizeof(
       f[2 * i] = p.x;
       f[2 * i + 1] = p.y;
     }
+  }
+}
+// The maximum of Q times 16 bytes of T (of 16-bit types two elements at a time).
+template <typename T, int Q>
+__device__ __forceinline__ float max_of(const uint4 (&v)[Q]) {
+  if constexpr (std::is_same_v<T, float>) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(v[q].x), __uint_as_float(v[q].y))), fmaxf(__uint_as_float(v[q].z), __uint_as_float(v[q].w)));
+    return m;
+  } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    auto as = [](const uint32_t& w) { return *reinterpret_cast<const T2*>(&w); };
+    T2 m = as(v[0].x);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) m = __hmax2(__hmax2(m, __hmax2(as(v[q].x), as(v[q].y))), __hmax2(as(v[q].z), as(v[q].w)));
+    return fmaxf(DT<T>::to_f(m.x), DT<T>::to_f(m.y));
   }
 }
 template <typename T>
@@ -328,7 +371,7 @@ __device__ __forceinline__ Coef coef_of(float a, float b, float g, int64_t t, fl
   const float scale = grad_base(w, in, c) / w.s;
   c.t = t >= 0 && t < in.vocab ? (int)t : -1;
   c.B = ENT ? -b * f * kLn2 * scale : 0.f;
-  c.A = -a * f * scale - (ENT ? c.B * (w.u / w.s) : 0.f);
+  c.A = -a * f * scale - (ENT ? c.B * w.mean : 0.f);
   c.at_t = grad_of<ENT>(xt, in.k, c) + a * f;
   c.masked = 0;
   return c;

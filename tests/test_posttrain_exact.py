@@ -160,3 +160,39 @@ def test_f16_rows_that_end_inside_a_vector(vocab, tau, level):
     # at a level of 65000 k m is rounded to 2^-8 / tau: one number for a row, so it does not show in log p or H
     assert ((lp - want).abs() <= tol(vocab) * (1 + want.abs())).all()
     assert ((h - wh).abs() <= 2 * tol(vocab) * (2 + wh + np.log(vocab))).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("gap", [1.0, 4.0, 8.0, 12.0, 20.0, 30.0, 45.0])
+def test_entropy_of_peaked_rows_with_unlikely_targets(gap, dtype):
+    """One token ``gap`` above all others, the target among those.  With the base b bits below the row's maximum, b
+    at most 10 or 0, log2 s and u / s are near b and off by a few of its roundings; the exponentials' error (2^-22 of what is not
+    the top token's share) and a row of 64 sums do not count beside H."""
+    g = torch.Generator(device="cuda").manual_seed(int(gap))
+    rows, vocab = 512, 64
+    x = (0.3 * torch.randn(rows, vocab, device="cuda", generator=g)).to(TORCH[dtype])
+    t = torch.randint(0, vocab - 1, (rows,), device="cuda", generator=g)
+    x[:, vocab - 1] = gap
+    want = softmax64(x)[2]
+    lp, h = token_logprobs(x, t, entropy=True)
+    out, _ = policy_loss_and_grad(x, t, lp, lp)
+    bits = min(10.0, gap / np.log(2)) + 1
+    err = (h.double() - want).abs()
+    assert (err <= 6 * U * (1 + bits) + 2.0**-18 * want).all(), f"{(err / U).max().item():.1f} u"
+    assert (h >= 0).all() and torch.equal(out.entropy, h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("below", [0.0, 5.0, 10.0, 20.0])
+def test_entropy_of_long_rows_with_unlikely_targets(below):
+    """32000 normal logits, the target ``below`` their mean: the same roundings as with a likely target.  H is near 11,
+    half a step there is 8 u; the sums' errors average out over a row's 128 partial sums to a few u of u / s, about
+    8: 32 u for the worst of 256 rows, 10 u in the mean."""
+    g = torch.Generator(device="cuda").manual_seed(int(below))
+    x = 2.0 * torch.randn(256, 32000, device="cuda", generator=g)
+    t = torch.randint(0, 32000, (256,), device="cuda", generator=g)
+    x[torch.arange(256), t] = -below
+    _, h = token_logprobs(x, t, entropy=True)
+    err = (h.double() - softmax64(x)[2]).abs() / U
+    assert err.max().item() <= 32 and err.mean().item() <= 10, (err.max().item(), err.mean().item())
