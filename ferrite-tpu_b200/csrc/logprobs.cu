@@ -94,7 +94,7 @@ struct LogprobsBwd {
     if ((threadIdx.x & 31) != 0) return 0.f;
     Row& w = *reinterpret_cast<Row*>(slot);
     const float2 v = stats[r];
-    w.w = Norm{v.x, fabsf(v.y), 0.f, !(v.y > 0.f)};
+    w.w = Norm{v.x, fabsf(v.y), 0.f, 0.f, !(v.y > 0.f)};
     w.a = p.t >= 0 && p.t < in.vocab ? (dlogp ? dlogp[r] : 0.f) : __int_as_float(0x7fc00000);
     w.b = 0.f;
     if constexpr (ENT) {

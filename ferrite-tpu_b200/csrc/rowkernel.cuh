@@ -59,10 +59,10 @@ struct Pad {
   static constexpr uint32_t kBits = std::is_same_v<T, float> ? (ENT ? 0xf149f2cau : 0xff800000u) : (ENT ? 0xf149f149u : 0xff80ff80u);
   static __device__ __forceinline__ uint4 vector() { return make_uint4(kBits, kBits, kBits, kBits); }
 };
-// Adds Q vectors to a state by one check of their sums.  What is left to do, vector by vector: nothing; their
+// Adds Q vectors to a state by one check of their sums.  BELOW: none of them is above the base.  What is left to do, vector by vector: nothing; their
 // part of u; or all of it.
 enum class Left { kNothing, kDot, kAll };
-template <class Op, typename T, int Q>
+template <class Op, bool BELOW, typename T, int Q>
 __device__ __forceinline__ Left push_usual(State& st, float nc, const uint4 (&raw)[Q], const Pairs2& kk) {
   uint64_t s2 = f2_make(0.f, 0.f), u2 = s2;
 #pragma unroll
@@ -75,10 +75,12 @@ __device__ __forceinline__ Left push_usual(State& st, float nc, const uint4 (&ra
   if (usual<Op::kLogp>(Op::kEnt ? fmaf(u, 0.f, s) : s)) {  // s, or NaN where u is
     st.s += s;
     if constexpr (Op::kEnt) st.u += u;
+    if (Op::kLogp && (BELOW || s <= kLowSum)) st.low += s;
     return Left::kNothing;
   }
   if (!Op::kEnt || !usual<Op::kLogp>(s)) return Left::kAll;
   st.s += s;
+  if (Op::kLogp && (BELOW || s <= kLowSum)) st.low += s;
   return Left::kDot;
 }
 
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
 #pragma unroll
           for (int q = 0; q < kShortVecs; ++q) raw[q] = !P::kThere || q * 32 < left ? ld_v4(at + q * 32 * N) : P::vector();
           if constexpr (Op::kLogp) raise<Op::kEnt>(st, nc, max_of<TI>(raw), in);
-          todo = push_usual<Op, TI>(st, nc, raw, kk);
+          todo = push_usual<Op, Op::kLogp, TI>(st, nc, raw, kk);
         }
         if (todo != Left::kNothing) {
 #pragma unroll 1
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
         push<Op::kEnt, Op::kLogp>(st, nc, one, in, kk);
       }
       __syncwarp();
-      w = normalise<Op::kEnt>(warp_merge<Op::kEnt>(st, in), in);
+      w = normalise<Op::kEnt>(warp_merge<Op::kEnt, Op::kLogp>(st, in), in);
     }
     const Coef cf = op.finish(r, w, in, g, slot);
     op.results(r, w, in, slot);
@@ -503,7 +505,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
           (void)wait_idle(&sh.states[h], parity, abort, 203);
           __syncwarp();
           const State st = lane < kWarps ? sh.warp_state[h][lane] : empty_state(sh.warp_state[h][0].m);
-          w = normalise<Op::kEnt>(warp_merge<Op::kEnt>(st, in), in);
+          w = normalise<Op::kEnt>(warp_merge<Op::kEnt, Op::kLogp>(st, in), in);
         } else {
           w = op.state(slot);
           // the passes have read the coefficients of this helper's row before
@@ -567,7 +569,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
             raw[q] = v[q * kGroup];  // past the row's end: whatever the chunk holds
             if (P::kThere && q * kGroup >= left) raw[q] = P::vector();
           }
-          todo = push_usual<Op, TI>(st, nc, raw, kk);
+          todo = push_usual<Op, false, TI>(st, nc, raw, kk);
         }
         if (todo != Left::kNothing) {
 #pragma unroll 1
@@ -588,7 +590,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
         push<Op::kEnt, Op::kLogp>(st, nc, one, in, kk);
       }
       __syncwarp();
-      st = warp_merge<Op::kEnt>(st, in);
+      st = warp_merge<Op::kEnt, Op::kLogp>(st, in);
       // the helper has read the states of its row before
       if constexpr (!GRAD) (void)mbar_wait(&sh.done[slot1.at], slot1.parity ^ 1, abort, 210);
       if (lane == 0) {

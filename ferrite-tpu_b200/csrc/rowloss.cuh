@@ -41,11 +41,17 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kBig = 65536.f;   // |k m| above this: y is k (x - m)
 constexpr float kHigh = 0x1p10f, kHuge = 0x1p80f;  // sums above this (an Op's) are redone against the maximum
 
-// (m, s, u): the base, sum of e and sum of e * y of the elements seen so far.
+// (m, s, u): the base, sum of e and sum of e * y of the elements seen so far; low: the part of s that is known to
+// come from elements at or below the base, or hardly above it.
 struct State {
-  float m, s, u;
+  float m, s, u, low;
 };
-__device__ __forceinline__ State empty_state(float base = -INFINITY) { return State{base, 0.f, 0.f}; }
+__device__ __forceinline__ State empty_state(float base = -INFINITY) { return State{base, 0.f, 0.f, 0.f}; }
+
+// The mean error of ex2.approx, relative and measured against f64 over 10^7 values an octave: -5.1e-8 below y = -1,
+// 3.4e-8 above y = 1, less between.  It is under half a step of f32, but sums of log-probabilities over long sequences
+// show what goes one way.  Of what is known to lie below the base it is taken out (logp_of, rebase).
+constexpr float kEx2Low = 5.1e-8f;
 
 // Rows whose results are asked for.
 struct RowIn {
@@ -92,12 +98,14 @@ __device__ __forceinline__ void rebase(State& st, float m, const RowIn& in) {
   }
   const float d = base_step(st.m, m, in), f = ex2_approx(d);
   if constexpr (ENT) st.u = f > 0.f && st.s != 0.f ? f * fmaf(st.s, d, st.u) : 0.f;
-  st.s = __fmul_rn(st.s, f);  // (never one fma with what is added to it: a row's s has the same bits in every kernel)
+  // s f (1 + kEx2Low), rounded once (and never one fma with what is added to it: a row's s has the same bits in every kernel)
+  st.s = fmaf(st.s, f, __fmul_rn(__fmul_rn(st.s, f), kEx2Low));
+  st.low = __fmul_rn(st.low, f);
   st.m = m;
 }
 
 // The states of a warp's lanes merged, in all lanes: one base (they usually have it), plain sums.
-template <bool ENT>
+template <bool ENT, bool LOGP>
 __device__ __forceinline__ State warp_merge(State st, const RowIn& in) {
   if (!__all_sync(0xffffffffu, st.m == __shfl_sync(0xffffffffu, st.m, 0))) {
     float m = st.m;
@@ -109,6 +117,7 @@ __device__ __forceinline__ State warp_merge(State st, const RowIn& in) {
   for (int off = 16; off > 0; off >>= 1) {
     st.s += __shfl_xor_sync(0xffffffffu, st.s, off);
     if constexpr (ENT) st.u += __shfl_xor_sync(0xffffffffu, st.u, off);
+    if constexpr (LOGP) st.low += __shfl_xor_sync(0xffffffffu, st.low, off);
   }
   return st;
 }
@@ -167,6 +176,8 @@ template <bool LOGP>
 __device__ __forceinline__ bool usual(float s) {
   return s < (LOGP ? kHigh : kHuge);
 }
+// A sum up to 2 has no element more than 1 above the base.
+constexpr float kLowSum = 2.f;
 template <int N>
 __device__ __forceinline__ float dot_masked(const float (&x)[N], float nc, const RowIn& in) {
   float u = 0.f;
@@ -201,7 +212,10 @@ __device__ __forceinline__ void push(State& st, float& nc, const float (&x)[N], 
           if (u != u) u = dot_masked(x, nc, in);
           st.u += u;
         }
-        if (!ENT || !dot) st.s += s;
+        if (!ENT || !dot) {
+          st.s += s;
+          if (LOGP && s <= kLowSum) st.low += s;
+        }
         return;
       }
       float cm = x[0];
@@ -214,9 +228,10 @@ __device__ __forceinline__ void push(State& st, float& nc, const float (&x)[N], 
   nc = minus_c(st.m, in);
 }
 
-// A finished row: base (c, or m where big), s, and the mean of y, u / s.
+// A finished row: base (c, or m where big), s, the mean of y, u / s, and the share of s that is known to be low
+// (the base's own element aside, whose 1 is exact).
 struct Norm {
-  float base, s, mean;
+  float base, s, mean, low;
   int big;
 };
 // Moves the power of two of s into the base, exactly: c2 = c + j is rounded, and what the rounding
@@ -224,31 +239,26 @@ struct Norm {
 template <bool ENT>
 __device__ __forceinline__ Norm normalise(const State& st, const RowIn& in) {
   const float c = __fmul_rn(st.m, in.k);
-  if (is_big(c) || !(st.s < INFINITY)) return Norm{is_big(c) ? st.m : c, st.s, ENT ? st.u / st.s : 0.f, is_big(c)};
+  if (is_big(c) || !(st.s < INFINITY)) return Norm{is_big(c) ? st.m : c, st.s, ENT ? st.u / st.s : 0.f, 0.f, is_big(c)};
   const uint32_t bits = __float_as_uint(st.s);
   const float l = (float)((int)(bits >> 23) - 127), f = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);  // s = 2^l f
   const float c2 = c + l, b = c2 - c, err = (c - (c2 - b)) + (l - b);  // c + l = c2 + err
   const float t = err * kLn2, s = fmaf(f, fmaf(0.5f * t, t, t), f);
-  if constexpr (!ENT) return Norm{c2, s, 0.f, 0};
-  const float inv = __fdividef(1.f, st.s), q = st.u * inv, rest = fmaf(-q, st.s, st.u) * inv;  // u / s = q + rest
-  return Norm{c2, s, (q - l) + (rest + err), 0};
+  const float inv = __fdividef(1.f, st.s), low = fmaxf(st.low - 1.f, 0.f) * inv;
+  if constexpr (!ENT) return Norm{c2, s, 0.f, low, 0};
+  const float q = st.u * inv, rest = fmaf(-q, st.s, st.u) * inv;  // u / s = q + rest
+  return Norm{c2, s, (q - l) + (rest + err), low, 0};
 }
 __device__ __forceinline__ float y_of(float x, const Norm& w, const RowIn& in) {
   return w.big ? (x - w.base) * in.k : fmaf(x, in.k_rest, fmaf(x, in.k_hi, -w.base));
 }
-// log p of one logit, rounded once: sums of it over long sequences show roundings that go one way, so
-// the difference is taken in f64.  The mean error of ex2.approx, measured against f64 over 10^7 values an
-// octave, is -5.1e-8 below y = -1 and 3.4e-8 above y = 1; s has it in all but the base's own term, so to first
-// order log p moves by the opposite times 1 - p.  Which of the two depends on how much of s lies above the
-// target: for logits of standard deviation 2.5 a normal distribution of log2(p vocab), here a logistic one.
-// log p is then off by 3.4e-8 at most on average, 6e-9 at tau 1 (tau 0.7 to 2, 256 to 131072 columns).
-constexpr float kEx2Below = -5.1e-8f, kEx2Above = 3.4e-8f;
+// log p of one logit, rounded once: the difference is taken in f64, and what is known of s's mean error (kEx2Low) is
+// taken out.  What is left of it is that of the part of s from elements above the base or in sums with such, if any:
+// within 5.1e-8 whatever the logits.
 __device__ __forceinline__ float logp_of(float xt, const Norm& w, const RowIn& in) {
   const double k = (double)in.k + (double)in.k_lo, l = (double)log2f(w.s);
   const double y = w.big ? fma((double)(xt - w.base), k, -l) : fma((double)xt, k, -(double)w.base) - l;
-  const float p = ex2_approx((float)y), ahead = (float)y + log2f((float)in.vocab);
-  const float below = 1.f / (1.f + ex2_approx(fminf(3.f - 2.f / 3.f * ahead, 100.f)));
-  return (float)(y * 0.6931471805599453 + (double)(fmaf(below, kEx2Below - kEx2Above, kEx2Above) * (1.f - p)));
+  return (float)fma(y, 0.6931471805599453, (double)(-kEx2Low * w.low));
 }
 __device__ __forceinline__ float entropy_of(const Norm& w) {
   const float h = (log2f(w.s) - w.mean) * kLn2;
