@@ -31,7 +31,6 @@ struct Distill {
   struct alignas(16) Row {
     uint32_t seen[kSeenWords];  // a bit for each token's hash
     float w;
-    float qlogq;   // sum_j q_j log2 q_j
     float bad;     // NaN if an index is out of range
     int16_t entries;  // 0: a masked row
     int16_t twice;    // a token is listed more than once
@@ -129,26 +128,21 @@ struct Distill {
       bad += __shfl_xor_sync(0xffffffffu, bad, off);
       first = fmaxf(first, __shfl_xor_sync(0xffffffffu, first, off));
     }
-    float sum = 0.f, dot = 0.f;
+    float sum = 0.f;
     for (int j = lane; j < top; j += 32) {
       const float y = (l.q[j] - m) * in.k;
       const float e = l.idx[j] >= 0 ? ex2_approx(y) : 0.f;
       l.q[j] = e;
       sum += e;
-      dot += e > 0.f ? e * y : (e != e ? e : 0.f);
     }
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      sum += __shfl_xor_sync(0xffffffffu, sum, off);
-      dot += __shfl_xor_sync(0xffffffffu, dot, off);
-    }
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     for (int j = lane; j < top; j += 32) l.q[j] /= sum;
     Row& row = *reinterpret_cast<Row*>(slot);
     __syncwarp();
     const bool twice = any_twice(row, l);
     if (lane == 0) {
       row.w = p.w;
-      row.qlogq = dot / sum - log2f(sum);
       row.bad = bad;
       row.entries = (int16_t)(bad != bad ? max(count, 1) : count);
       row.twice = twice;
@@ -171,14 +165,19 @@ struct Distill {
     const List l = list(slot);
     const Row& row = *reinterpret_cast<const Row*>(slot);
     const int lane = threadIdx.x & 31;
-    const float ls = log2f(w.s);
+    // sum q (log q - log p), each difference taken in f64 before the sum: as the student nears the teacher they are
+    // small beside the two logarithms
+    const double k = (double)in.k + (double)in.k_lo, ls = (double)log2f(w.s);
     float part = 0.f;
     for (int j = lane; j < top; j += 32)
-      if (l.idx[j] >= 0 && l.q[j] != 0.f) part += l.q[j] * (y_of(l.x[j], w, in) - ls);
+      if (l.idx[j] >= 0 && l.q[j] != 0.f) {
+        const double y = w.big ? (double)(l.x[j] - w.base) * k : fma((double)l.x[j], k, -(double)w.base);
+        part = fmaf(l.q[j], (float)((double)log2f(l.q[j]) + (ls - y)), part);
+      }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) part += __shfl_xor_sync(0xffffffffu, part, off);
     if (lane == 0) {
-      const float per = row.entries ? tau * tau * kLn2 * (row.qlogq - part) + row.bad : 0.f;
+      const float per = row.entries ? tau * tau * kLn2 * part + row.bad : 0.f;
       per_token[r] = per;
       terms[r] = row.entries ? row.w * per : 0.f;
     }

@@ -249,9 +249,6 @@ __device__ __forceinline__ Norm normalise(const State& st, const RowIn& in) {
   const float q = st.u * inv, rest = fmaf(-q, st.s, st.u) * inv;  // u / s = q + rest
   return Norm{c2, s, (q - l) + (rest + err), low, 0};
 }
-__device__ __forceinline__ float y_of(float x, const Norm& w, const RowIn& in) {
-  return w.big ? (x - w.base) * in.k : fmaf(x, in.k_rest, fmaf(x, in.k_hi, -w.base));
-}
 // log p of one logit, rounded once: the difference is taken in f64, and what is known of s's mean error (kEx2Low) is
 // taken out.  What is left of it is that of the part of s from elements above the base or in sums with such, if any:
 // within 5.1e-8 whatever the logits.

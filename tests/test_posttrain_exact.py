@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from ferrite import _native as nat
+from ferrite.kernels.distillation import distillation_loss, distillation_loss_reference
 from ferrite.kernels.logprobs import token_logprobs
 from ferrite.kernels.policy_loss import policy_loss, policy_loss_and_grad
 from ferrite.kernels.preference_loss import preference_loss_and_grad
@@ -232,3 +233,20 @@ def test_mean_error_of_logprobs(name, vocab, tau):
         err.append(lp.double() - softmax64(x, tau)[0].gather(1, t[:, None])[:, 0])
     err = torch.cat(err)
     assert abs(err.mean().item()) <= 5.1e-8 + 4 * err.std().item() / len(err) ** 0.5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tau", [1.0, 2.0])
+def test_distillation_near_the_teacher(tau):
+    """Where the student has almost learned the lists, the KL is a sum of small differences: no less exact than plain f32
+    operations, which take the differences before the sum."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rows, vocab, top = 4096, 512, 256
+    x = 3 * torch.randn(rows, vocab, device="cuda", generator=g)
+    v, idx = x.topk(top)
+    v = v + 0.02 * torch.randn(rows, top, device="cuda", generator=g)
+    lq, lp = torch.log_softmax(v.double() / tau, 1), torch.log_softmax(x.double() / tau, 1).gather(1, idx)
+    want = tau**2 * (lq.exp() * (lq - lp)).sum(1)
+    plain = distillation_loss_reference(x, v, idx, temperature=tau).per_token.double() - want
+    own = distillation_loss(x, v, idx, temperature=tau).per_token.double() - want
+    assert own.pow(2).mean().sqrt() <= plain.pow(2).mean().sqrt(), (own.pow(2).mean().sqrt().item(), plain.pow(2).mean().sqrt().item())
