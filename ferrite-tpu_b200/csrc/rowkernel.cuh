@@ -87,15 +87,15 @@ __device__ __forceinline__ Left push_usual(State& st, float nc, const uint4 (&ra
 // --------------------------------------------------------------------------
 // Short rows: a warp per row, which reads it twice (the second time from L1 or L2).  No barriers; many
 // rows in flight hide the latency of each.  Bound by that latency and by the work of a row that does
-// not grow with it.  From 16 KB on the two are close (policy, 16384 x 8192 bf16: 132 us
-// against the other kernel's 136) and the other's copies keep up with longer rows; half as long rows take 68 us
-// against its 126.
+// not grow with it.  The other kernel's copies keep up with longer rows.  Where they meet (us, this kernel and the other;
+// policy, log-probabilities, lists of 64): 16384 rows of 16 KB, bf16 125 and 130, 49 and 57, 145 and 186, f32 policy 93 and 131; of 18 KB,
+// f16 policy 151 and 162; 8192 rows of 24 KB, bf16 106 and 106, 39 and 48, 126 and 110, f32 with entropy bonus 101 and 89; of 28 KB 124 and 110.
 // --------------------------------------------------------------------------
 
 constexpr int kShortWarps = 4;                 // rows of a CTA
 constexpr int kShortSlots = 48 * 1024;         // shared memory that their ops may take
 constexpr int kShortVecs = 4;                  // vectors a lane asks for at a time
-constexpr int kShortRow = 16384;               // bytes: rows from this on go to the kernel for whole CTAs
+constexpr int kShortRow = 20 * 1024;           // bytes: longer rows go to the kernel for whole CTAs
 
 template <class Op, typename TI, typename TO, bool GRAD>
 __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, RowOut out, Op op) {
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
 }
 
 // --------------------------------------------------------------------------
-// Rows of 16 KB and more: one read from HBM, one write.
+// Rows over 20 KB: one read from HBM, one write.
 //
 // Bound: HBM.  Both passes over a row (the sums, then the gradient) stream it through shared memory,
 // the second one from L2, where the rows in flight stay (296 CTAs x 125 KB, 592 x 62.5 KB are 37 MB): the first
@@ -226,9 +226,12 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
 //     of them takes about 600 cycles a copy -- its waits and its issue, one after the other -- and
 //     held reads to 3.7 TB/s with 8 KB copies.)
 //   - kGroups groups of four warps (one to each of the SM's quarters) run the passes, each on chunks
-//     of its own in turn.  The second pass of shorter rows runs one row behind the first (lag), so that
-//     nothing waits for what lies between a row's two passes (two CTAs, 8192 x 32000 bf16: 201 us, else
-//     207); with longer rows the two of each CTA no longer stay in L2 together (f32: 324 us, else 272);
+//     of its own in turn.  The second pass of shorter f32 rows runs one row behind the first (lag), so that
+//     nothing waits for what lies between a row's two passes; with longer rows the two of each CTA no longer stay in
+//     L2 together, all the less the more gradient goes through it.  Policy, 8192 rows (us, with and without lag):
+//     bf16 gradient 8000 columns 90 and 98, 15000 130 and 142, 16384 140 and 143; f32 gradient 8000 columns 97 and 111, 10000 117
+//     and 130, 12000 144 and 136, 16384 208 and 180.  16-bit rows have four CTAs an SM, which fill each other's gaps: 16384 x 8192
+//     130 and 135, but 8192 x 16384 114 and 114, with the bonus 123 and 121, with lists 146 and 128; they run without;
 //   - that is the work of kHelpers warps, rows in turn: fetch what the row's loss needs besides the
 //     logits (ahead of time), merge the passes' states, hand back the gradient's coefficients, write
 //     the row's results, and at last the single entries of a list.
@@ -237,18 +240,16 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_row_kernel(RowIn in, R
 // --------------------------------------------------------------------------
 
 // How the kernel is laid out: GROUPS of four warps for the passes, a copy warp for each, HELPERS, and
-// CTAS of these to an SM; chunks of CHUNK bytes, PLACES of them in the ring; LAG: rows up to so many
-// bytes run with the second pass one row behind the first.
+// CTAS of these to an SM; chunks of CHUNK bytes, PLACES of them in the ring; LAG: rows whose bytes and twice their
+// gradient's come to no more run with the second pass one row behind the first.
 //
 // A helper has one place for its row's coefficients.  It writes row i's once every warp has handed in the states
 // of row i, so every warp must have read those of its row before by then, row i - HELPERS.  Without lag a warp
 // reads row i - 1's ahead of the states of row i.  With lag its order is first(i - 1), second(i - 2), first(i): it has
-// read those of row i - 2 and not yet those of row i - 1, so that two helpers are needed, or a helper that waits
-// until its row's gradient is written before it goes on to its next (lists).
-template <int GROUPS, int HELPERS, int CTAS, int CHUNK, int PLACES, int64_t LAG, bool WAITS>
+// read those of row i - 2 and not yet those of row i - 1, so that two helpers are needed.
+template <int GROUPS, int HELPERS, int CTAS, int CHUNK, int PLACES, int64_t LAG>
 struct Layout {
-  static_assert(LAG == 0 || HELPERS >= 2 || WAITS, "the coefficients of a row behind would be overwritten");
-  static constexpr bool kWaits = WAITS;
+  static_assert(LAG == 0 || HELPERS >= 2, "the coefficients of a row behind would be overwritten");
   static constexpr int kGroups = GROUPS, kHelpers = HELPERS, kCtas = CTAS, kChunk = CHUNK, kPlaces = PLACES;
   static constexpr int64_t kLag = LAG;
   static constexpr int kGroup = 128;                        // threads of a group
@@ -265,12 +266,13 @@ struct Layout {
 };
 // 16-bit rows up to 128 KB, four CTAs of one group: what a row costs whatever its length is paid by four warps
 // instead of eight, and three other CTAs fill the gaps (policy 8192 x 32000 bf16: 189 us against 200 for the
-// other layout, 8192 x 16384 109 against 125; 1000 x 131072 127 against 115).  Lists take 8 KB chunks
+// other layout, 1000 x 131072 127 against 115).  A second helper keeps the sums of short rows going (log-probabilities 16384 x 8192
+// bf16: 54 us against 68 with one); lists have no room for it.  Lists take 8 KB chunks
 // (distill 8192 x 32000 bf16: 200 us against 207 with 16 KB; policy 197 against 189).
 template <bool LIST>
-using NarrowLayout = Layout<1, LIST ? 1 : 2, 4, LIST ? 8192 : 16384, LIST ? 6 : 3, 33 * 1024, LIST>;
+using NarrowLayout = Layout<1, LIST ? 1 : 2, 4, LIST ? 8192 : 16384, LIST ? 6 : 3, 0>;
 // Longer rows, and f32 rows, which have half the work to the byte (policy 8192 x 32000 f32: 259 us against 292).
-using WideLayout = Layout<2, 2, 2, 16384, 6, 64 * 1024, false>;
+using WideLayout = Layout<2, 2, 2, 16384, 6, 128 * 1024>;
 constexpr int64_t kNarrowRow = 128 * 1024;
 
 template <class L>
@@ -379,7 +381,6 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
   constexpr int kGroup = L::kGroup, kPass = L::kPass, kWarps = L::kWarps, kVecPer = L::kVecPer;
   constexpr bool kSums = !Op::kHasStats;        // a first pass
   constexpr bool kFix = GRAD && Op::kList;
-  static_assert(!L::kWaits || Op::kList, "a layout that counts on its helpers' wait for the gradient");
   extern __shared__ __align__(128) char smem[];
   RingShared<L>& sh = *reinterpret_cast<RingShared<L>*>(smem);
   char* ring = smem + ring_header<L>();
@@ -719,7 +720,8 @@ static cudaError_t launch_ring(cudaStream_t s, const RowIn& in, const RowOut& ou
   places = (places < L::kPlaces ? places : L::kPlaces) / L::kGroups * L::kGroups;
   const size_t smem = (size_t)ring_header<L>() + (size_t)places * L::kChunk + slots;
   const int64_t bytes = in.vocab * (int64_t)sizeof(TI), ctas = (int64_t)num_sms(dev) * (bytes <= kPairRow ? L::kCtas : 1);
-  return launch_pdl(kern, dim3((unsigned)(in.rows < ctas ? in.rows : ctas)), dim3(L::kThreads), smem, s, in, out, op, places, bytes <= L::kLag);
+  return launch_pdl(kern, dim3((unsigned)(in.rows < ctas ? in.rows : ctas)), dim3(L::kThreads), smem, s, in, out, op, places,
+                    GRAD && bytes + 2 * in.vocab * (int64_t)sizeof(TO) <= L::kLag);
 }
 
 template <class Op, typename TI, typename TO, bool GRAD>
@@ -732,7 +734,7 @@ static int launch_row(cudaStream_t s, const RowIn& in, const RowOut& out, const 
   // gradient or without: so a row's results have the same bits in every call (log-probabilities taken
   // in one batch and compared in another differ by nothing), as long as it starts on a 16-byte boundary.
   const int64_t bytes = in.vocab * (int64_t)sizeof(TI);
-  if (bytes < kShortRow && kShortWarps * slot <= kShortSlots) {
+  if (bytes <= kShortRow && kShortWarps * slot <= kShortSlots) {
     const int64_t ctas = (in.rows + kShortWarps - 1) / kShortWarps, most = (int64_t)num_sms(dev) * 16;
     e = launch_pdl(short_row_kernel<Op, TI, TO, GRAD>, dim3((unsigned)(ctas < most ? ctas : most)), dim3(kShortWarps * 32), kShortWarps * slot, s,
                    in, out, op);
