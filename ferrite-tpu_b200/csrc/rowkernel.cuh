@@ -266,11 +266,12 @@ struct Layout {
 };
 // 16-bit rows up to 128 KB, four CTAs of one group: what a row costs whatever its length is paid by four warps
 // instead of eight, and three other CTAs fill the gaps (policy 8192 x 32000 bf16: 189 us against 200 for the
-// other layout, 1000 x 131072 127 against 115).  A second helper keeps the sums of short rows going (log-probabilities 16384 x 8192
-// bf16: 54 us against 68 with one); lists have no room for it.  Lists take 8 KB chunks
-// (distill 8192 x 32000 bf16: 200 us against 207 with 16 KB; policy 197 against 189).
+// other layout, 1000 x 131072 127 against 115).  One helper: a second one helps sums alone (log-probabilities 8192 x 32000
+// bf16: 84 us against 90), and costs where a gradient is written (policy with bonus, 8192 x 12000: 118 against 114) or follows in
+// the next launch (preference 16384 x 32000, a third masked: 483 against 454).  Lists take 8 KB chunks (distill 8192 x 32000 bf16: 200 us against
+// 207 with 16 KB; policy 197 against 189).
 template <bool LIST>
-using NarrowLayout = Layout<1, LIST ? 1 : 2, 4, LIST ? 8192 : 16384, LIST ? 6 : 3, 0>;
+using NarrowLayout = Layout<1, 1, 4, LIST ? 8192 : 16384, LIST ? 6 : 3, 0>;
 // Longer rows, and f32 rows, which have half the work to the byte (policy 8192 x 32000 f32: 259 us against 292).
 using WideLayout = Layout<2, 2, 2, 16384, 6, 128 * 1024>;
 constexpr int64_t kNarrowRow = 128 * 1024;

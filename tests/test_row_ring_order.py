@@ -24,22 +24,25 @@ SOURCE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))
 WARPS, ROWS = 2, 5
 
 
-def _value(text, is_list):
-    m = re.fullmatch(r"\s*LIST \? (.+?) : (.+)", text)
-    # numbers, products of numbers, truth values
-    return eval((m.group(1) if is_list else m.group(2)) if m else text, {"LIST": is_list, "false": False, "true": True})
+def _value(text, lists, grad):
+    m = re.fullmatch(r"\s*(.+) \? (.+?) : (.+)", text)
+    names = {"LIST": lists, "GRAD": grad, "false": False, "true": True}
+    if m:
+        text = m.group(2) if eval(m.group(1).replace("||", "or"), names) else m.group(3)
+    return eval(text, names)  # a number, or a product of numbers
 
 
 def layouts():
-    """(name, lists, helpers, lag) of every layout in the source."""
+    """(name, lists, grad, helpers, lag) of every layout in the source."""
     src = open(SOURCE).read()
     names = re.search(r"template <([^>]*)>\nstruct Layout", src).group(1)
     at = {n.split()[-1]: i for i, n in enumerate(names.split(","))}
     out = []
     for name, args in re.findall(r"^using (\w+) = Layout<(.*)>;", src, re.M):
-        for is_list in (False, True):
-            v = [_value(a, is_list) for a in args.split(",")]
-            out.append((name, is_list, v[at["HELPERS"]], v[at["LAG"]] > 0))
+        for lists in (False, True):
+            for grad in (False, True):
+                v = [_value(a, lists, grad) for a in args.split(",")]
+                out.append((name, lists, grad, v[at["HELPERS"]], v[at["LAG"]] > 0))
     return out
 
 
@@ -131,13 +134,12 @@ def faults(progs):
     return None
 
 
-@pytest.mark.parametrize("name,lists,helpers,lag", layouts())
-@pytest.mark.parametrize("kind", ["gradient", "forward", "saved statistics"])
-def test_every_order_of_a_layout(name, lists, helpers, lag, kind):
-    if kind == "saved statistics" and lists:
-        pytest.skip("no operator with lists takes saved statistics")
+@pytest.mark.parametrize("name,lists,grad,helpers,lag", layouts())
+def test_every_order_of_a_layout(name, lists, grad, helpers, lag):
     for late in {False, lag}:  # rows longer than the layout's limit run without lag
-        assert faults(programs(kind != "forward", kind.startswith("saved"), late, lists, helpers)) is None
+        assert faults(programs(grad, False, late, lists, helpers)) is None
+    if grad and not lists:
+        assert faults(programs(grad, True, False, lists, helpers)) is None  # from saved statistics
 
 
 def test_the_model_finds_what_is_wrong():
