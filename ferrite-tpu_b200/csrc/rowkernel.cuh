@@ -86,7 +86,8 @@ __device__ __forceinline__ Left push_usual(State& st, float nc, const uint4 (&ra
 
 // --------------------------------------------------------------------------
 // Short rows: a warp per row, which reads it twice (the second time from L1 or L2).  No barriers; many
-// rows in flight hide the latency of each.  Bound by that latency and by the work of a row that does
+// rows in flight hide the latency of each.  Where log p is asked for, a lane raises its base to the maximum of the
+// vectors that it has just fetched (16384 x 4096 bf16: policy 68 -> 65 us, log-probabilities 34 -> 29).  Bound by that latency and by the work of a row that does
 // not grow with it.  The other kernel's copies keep up with longer rows.  Where they meet (us, this kernel and the other;
 // policy, log-probabilities, lists of 64): 16384 rows of 16 KB, bf16 125 and 130, 49 and 57, 145 and 186, f32 policy 93 and 131; of 18 KB,
 // f16 policy 151 and 162; 8192 rows of 24 KB, bf16 106 and 106, 39 and 48, 126 and 110, f32 with entropy bonus 101 and 89; of 28 KB 124 and 110.
@@ -651,9 +652,12 @@ __global__ void __launch_bounds__(L::kThreads, L::kCtas) ring_kernel(RowIn in, R
                 store_at(to + q * kGroup * N, d, vec);
               }
           }
-          // Released after the chunk's last use: its stores have what the loads brought, as in the first
-          // pass the check of the sums has.  Released right after the loads were issued, the next copy
-          // overtook some of them.
+          // Released after the chunk's last use.  The arrival orders this warp's accesses of shared memory among
+          // ordinary ones, but the next copy writes through the async proxy, and nothing orders that after loads that
+          // are still under way: released right after the loads were issued, the copy overtook some of them.  A store
+          // that needs a loaded value (in the first pass, the branch on the check of the sums) is not issued before the
+          // value is there, and the arrival follows it.  A proxy fence before the arrival would do as well, but waits for more:
+          // log-probabilities 8192 x 32000 bf16 took 94 us with it for 89, 2999 x 50257 f16 66 for 57.
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.empty[at.at]);
           at.next(ring_chunks, kGroups);

@@ -23,8 +23,8 @@
 // a unit of a y of 4 or more and would be rounded away each time; positive, because -inf times a rest
 // of 0 or below would be NaN.  Where |c| passes
 // 2^16 (logits in the tens of thousands, rows of the type's lowest value, infinities) y_i is
-// k (x_i - m) with m the maximum.  At its end a row is normalised: c takes up log2 s, so that s is
-// 1 but for rounding and log p = ln2 y loses nothing to cancellation.  A logit of -inf has e_i = 0
+// k (x_i - m) with m the maximum.  At its end a row is normalised: c takes up the power of two of s, so that s lies in
+// [1, 2) and its logarithm is small beside y.  A logit of -inf has e_i = 0
 // and contributes nothing; NaN and +inf make the row's results NaN.
 #pragma once
 

@@ -2,8 +2,8 @@
 
 The scores that post-training needs next to the training loss: those of the tokens that
 were sampled or written, under the model that is trained, the one that sampled them, or a
-frozen reference.  One read of the logits (``ferrite_logprobs_fwd``: a running maximum and
-rescaled sums, f32 whatever the logits' type); the backward (``ferrite_logprobs_bwd``)
+frozen reference.  One read of the logits (``ferrite_logprobs_fwd``: sums of exponentials
+against a base near the row's top, f32 whatever the logits' type); the backward (``ferrite_logprobs_bwd``)
 reads them once more and writes the gradient in their type.  No counterpart in the
 reference, whose only loss is the mean cross-entropy (src/ferrite/model/gpt.py:147-152).
 """
