@@ -85,8 +85,11 @@ def check_temperature(temperature: float) -> float:
     return temperature
 
 
-def upstream(g: torch.Tensor) -> torch.Tensor:
-    """The gradient of a scalar loss as a dense f32 device scalar."""
+def upstream(g: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
+    """The gradient of a scalar loss as a dense f32 scalar on the logits' device."""
+    if g.numel() != 1 or not g.is_floating_point():
+        raise ValueError(f"the upstream gradient must be one floating-point number, got {g.dtype} of shape {tuple(g.shape)}")
+    same_device(logits, g)
     return g.detach().reshape(()).to(torch.float32).contiguous()
 
 

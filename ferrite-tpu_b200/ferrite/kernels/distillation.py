@@ -74,7 +74,7 @@ class _Distillation(torch.autograd.Function):
     def backward(ctx, g, *_):
         # statistics and gradient in one launch, as in the policy loss
         logits, values, indices, weights = ctx.saved_tensors
-        _, grad = _launch(logits, values, indices, weights, ctx.temperature, logits.dtype, _rows.upstream(g), 1.0)
+        _, grad = _launch(logits, values, indices, weights, ctx.temperature, logits.dtype, _rows.upstream(g, logits), 1.0)
         return _rows.first_only(grad, logits, g), None, None, None, None
 
 
@@ -103,7 +103,7 @@ def distillation_loss_and_grad(logits, teacher_values, teacher_indices, weights=
     on the device, multiplies the gradient as well, before it is rounded."""
     grad_dtype = grad_dtype or logits.dtype
     values, indices, weights, temperature = _check(logits, teacher_values, teacher_indices, weights, temperature, grad_dtype)
-    dloss = None if upstream is None else _rows.upstream(upstream)
+    dloss = None if upstream is None else _rows.upstream(upstream, logits)
     return _launch(logits, values, indices, weights, temperature, grad_dtype, dloss, float(grad_scale))
 
 

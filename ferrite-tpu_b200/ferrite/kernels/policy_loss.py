@@ -78,7 +78,7 @@ class _PolicyLoss(torch.autograd.Function):
         # the row's statistics again and the gradient, in one launch: as much traffic as
         # reading the logits for the gradient alone
         logits, targets, *rest = ctx.saved_tensors
-        _, grad = _launch(logits, targets, rest, *ctx.args, logits.dtype, _rows.upstream(g), 1.0)
+        _, grad = _launch(logits, targets, rest, *ctx.args, logits.dtype, _rows.upstream(g, logits), 1.0)
         return _rows.first_only(grad, logits, g), None, None, None, None, None, None
 
 
@@ -110,7 +110,7 @@ def policy_loss_and_grad(logits, targets, old_logprobs, advantages, weights=None
     on the device, multiplies the gradient as well, before it is rounded."""
     grad_dtype = grad_dtype or logits.dtype
     targets, rest, temperature = _check(logits, targets, old_logprobs, advantages, weights, ref_logprobs, clip_low, clip_high, temperature, grad_dtype)
-    dloss = None if upstream is None else _rows.upstream(upstream)
+    dloss = None if upstream is None else _rows.upstream(upstream, logits)
     return _launch(logits, targets, rest, (float(clip_low), float(clip_high)), (float(kl_coef), float(entropy_coef)), temperature,
                    int(ignore_index), grad_dtype, dloss, float(grad_scale))
 

@@ -92,7 +92,7 @@ class _Preference(torch.autograd.Function):
     @nat.on_tensor_device
     def backward(ctx, g, *_):
         logits, targets, stats, coef = ctx.saved_tensors
-        grad = logprobs_backward(logits, targets, stats, None, coef, None, _rows.upstream(g), 1.0, ctx.temperature, ctx.ignore_index, logits.dtype)
+        grad = logprobs_backward(logits, targets, stats, None, coef, None, _rows.upstream(g, logits), 1.0, ctx.temperature, ctx.ignore_index, logits.dtype)
         return (_rows.first_only(grad, logits, g), *([None] * 9))
 
 
@@ -124,10 +124,11 @@ def preference_loss_and_grad(logits, targets, ref_logprobs, offsets, *, beta: fl
     the gradient as well, before it is rounded."""
     grad_dtype = grad_dtype or logits.dtype
     targets, ref, offsets, temperature = _check(logits, targets, ref_logprobs, offsets, beta, kind, label_smoothing, temperature, grad_dtype)
+    dloss = None if upstream is None else _rows.upstream(upstream, logits)
     out, stats, coef, grad = _launch(logits, targets, ref, offsets, float(beta), kind, float(label_smoothing), average, temperature, int(ignore_index),
-                                     True, grad_dtype if upstream is None else None, float(grad_scale))
-    if upstream is not None:
-        grad = logprobs_backward(logits, targets, stats, None, coef, None, _rows.upstream(upstream), float(grad_scale), temperature, int(ignore_index), grad_dtype)
+                                     True, grad_dtype if dloss is None else None, float(grad_scale))
+    if dloss is not None:
+        grad = logprobs_backward(logits, targets, stats, None, coef, None, dloss, float(grad_scale), temperature, int(ignore_index), grad_dtype)
     return out, grad
 
 

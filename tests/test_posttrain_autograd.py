@@ -4,10 +4,10 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
-from ferrite.kernels.distillation import distillation_loss
+from ferrite.kernels.distillation import distillation_loss, distillation_loss_and_grad
 from ferrite.kernels.logprobs import token_logprobs
-from ferrite.kernels.policy_loss import policy_loss
-from ferrite.kernels.preference_loss import preference_loss
+from ferrite.kernels.policy_loss import policy_loss, policy_loss_and_grad
+from ferrite.kernels.preference_loss import preference_loss, preference_loss_and_grad
 from ferrite.kernels.tied_head import tied_head_distillation_loss, tied_head_policy_loss, tied_head_preference_loss
 
 
@@ -102,3 +102,21 @@ def test_second_derivatives_are_refused():
         with pytest.raises(RuntimeError, match="no second derivative"):
             (g.pow(2).sum() + at.sum()).backward()
             pytest.fail(f"loss {n}: the second derivative was dropped")
+
+
+@pytest.mark.gpu
+def test_upstream_scalars():
+    """``upstream`` is a number on the logits' device, and multiplies the gradient like ``grad_scale``."""
+    x, t, f, off, v, i = _inputs("cuda", grad=False)
+    calls = [
+        lambda **kw: policy_loss_and_grad(x, t, f, f, **kw),
+        lambda **kw: preference_loss_and_grad(x, t, f, off, **kw),
+        lambda **kw: distillation_loss_and_grad(x, v, i, **kw),
+    ]
+    for call in calls:
+        for bad in (torch.tensor(2.0), torch.ones(2, device="cuda"), torch.ones((), device="cuda", dtype=torch.long)):
+            with pytest.raises((ValueError, RuntimeError)):
+                call(upstream=bad)
+        out, grad = call(upstream=torch.tensor([4.0], device="cuda", dtype=torch.float64))
+        want, scaled = call(grad_scale=4.0)
+        assert torch.equal(grad, scaled) and torch.equal(out.loss, want.loss)
