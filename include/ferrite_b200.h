@@ -269,8 +269,8 @@ FERRITE_API int ferrite_xent_bwd(void* stream, const float* logits, const void* 
  *     with row stride ld_out; it must not overlap logits.  The gradient is that of the loss
  *     times (*dloss) * scale (dloss a device scalar, NULL meaning 1).
  *   - a row's results do not depend on the call's other rows: the same logits, target and
- *     temperature give the same bits in any batch, with a gradient or without, wherever the
- *     row starts on a 16-byte boundary.
+ *     temperature give the same bits in any batch, with a gradient or an entropy or without,
+ *     wherever the row starts on a 16-byte boundary.
  *   - statistics, sums and losses are f32 (sums over rows are accumulated in f64, in a
  *     fixed order: results do not change from run to run).
  *   - a logit of -inf has p = 0 exactly; NaN or +inf makes the row's results NaN. */

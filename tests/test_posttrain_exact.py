@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from ferrite import _native as nat
-from ferrite.kernels.distillation import distillation_loss, distillation_loss_reference
+from ferrite.kernels.distillation import distillation_loss, distillation_loss_and_grad, distillation_loss_reference
 from ferrite.kernels.logprobs import token_logprobs
 from ferrite.kernels.policy_loss import policy_loss, policy_loss_and_grad
 from ferrite.kernels.preference_loss import preference_loss_and_grad
@@ -250,3 +250,63 @@ def test_distillation_near_the_teacher(tau):
     plain = distillation_loss_reference(x, v, idx, temperature=tau).per_token.double() - want
     own = distillation_loss(x, v, idx, temperature=tau).per_token.double() - want
     assert own.pow(2).mean().sqrt() <= plain.pow(2).mean().sqrt(), (own.pow(2).mean().sqrt().item(), plain.pow(2).mean().sqrt().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,dtype", [(6000, 5003, "f16"), (4000, 12345, "bf16"), (2500, 32003, "bf16"), (2000, 12001, "f32"), (1200, 32001, "f32"), (700, 70001, "f16"), (400, 90001, "f32")])
+def test_every_entry_where_the_gpu_is_full(rows, vocab, dtype):
+    """Several rows to a CTA in every kernel and layout, off 16-byte boundaries, some masked: every entry of the gradients of
+    log-probabilities with entropies, of pairs and of distillation, and the same bits again.  An entry is off by tol of each
+    of its parts (and its coefficient's own error), and the store."""
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = (3 * torch.randn(rows, vocab, device="cuda", generator=g)).to(TORCH[dtype])
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    t[torch.rand(rows, device="cuda", generator=g) < 0.15] = IGN
+    live = t != IGN
+    a, b = torch.randn(2, rows, device="cuda", generator=g)
+    ref = torch.randn(rows, device="cuda", generator=g) - 10
+    pairs = 4
+    off = torch.linspace(0, rows - 3, 2 * pairs + 1, device="cuda").long()
+    top = 40
+    v, idx = torch.randn(rows, top, device="cuda", generator=g), torch.randint(0, vocab, (rows, top), device="cuda", generator=g)
+    w = torch.rand(rows, device="cuda", generator=g) * (torch.rand(rows, device="cuda", generator=g) > 0.15)
+
+    def logprobs():
+        leaf = x.detach().requires_grad_(True)
+        return torch.autograd.grad(token_logprobs(leaf, t, entropy=True), leaf, (a, b))[0]
+
+    grads = [logprobs(), preference_loss_and_grad(x, t, ref, off, kind="squared", average=True)[1], distillation_loss_and_grad(x, v, idx, w, temperature=2.0)[1]]
+    again = [logprobs(), preference_loss_and_grad(x, t, ref, off, kind="squared", average=True)[1], distillation_loss_and_grad(x, v, idx, w, temperature=2.0)[1]]
+    assert all(torch.equal(p, q) for p, q in zip(grads, again))
+    # the pairs' coefficients: h is a difference of means of logp - ref, dL / dh = 2 (h - 5)
+    step = [(r, min(rows, r + 400)) for r in range(0, rows, 400)]
+    logp = torch.cat([softmax64(x[r:q])[0].gather(1, t[r:q].clamp_min(0)[:, None])[:, 0] for r, q in step])
+    at = torch.arange(rows, device="cuda")
+    inside = (at >= off[:-1, None]) & (at < off[1:, None]) & live
+    count = inside.sum(1).clamp_min(1)
+    d = torch.where(inside, logp - ref.double(), 0.0).sum(1) / count
+    dh = 2 * (d[0::2] - d[1::2] - 5) / pairs
+    slope = torch.stack([dh, -dh], 1).reshape(-1) / count
+    co = (inside * slope[:, None]).sum(0)
+    # logp's error in the mean, and the roundings of h and of the coefficient
+    shaky = (inside * (2 / pairs / count * 2 * (tol(vocab) * 40 + 8 * U * 40))[:, None]).sum(0) + 8 * U * co.abs()
+    for r, q in step:
+        s = slice(r, q)
+        lp, p, h = softmax64(x[s])
+        one = torch.zeros_like(p)
+        one[torch.arange(q - r, device="cuda"), t[s].clamp_min(0)] = 1.0
+        on = live[s, None]
+        ent = p * (lp.clamp_min(-1e5) + h[:, None])
+        at_, bt, ct = a[s, None].double(), b[s, None].double(), co[s, None]
+        want = torch.where(on, at_ * (one - p) - bt * ent, 0.0)
+        bound = 2 * tol(vocab) * (at_.abs() * (p + one) + bt.abs() * p * (lp.abs() + 3 * h[:, None] + 2)) + 4 * U * at_.abs() * one
+        wanted = [(want, bound), (torch.where(on, ct * (one - p), 0.0), (2 * tol(vocab) * ct.abs() + shaky[s, None]) * (p + one))]
+        lq = torch.log_softmax(v[s].double() / 2, 1)
+        p2 = softmax64(x[s], 2.0)[1]
+        q2 = torch.zeros_like(p2).scatter_add_(1, idx[s], lq.exp())
+        wt = 2 * w[s, None].double()
+        wanted.append((wt * (p2 - q2), 2 * wt * (p2 + q2) * (tol(vocab) + tol(64 * top))))
+        for n, ((want, bound), got) in enumerate(zip(wanted, grads)):
+            bad = (got[s].double() - want).abs() > bound + 1.01 * stored(want, got.dtype)
+            assert not bad.any(), f"gradient {n}: {int(bad.sum())} entries off, the first in row {r + int(bad.any(1).nonzero()[0])}"
+    nat.device_status()
